@@ -1,0 +1,80 @@
+/*
+ * qf_attn.h -- the key/value cache of a layer's sequences and the attention of
+ * their newest rows over it: what fork rows (up to 64 drafted tokens of one
+ * sequence, a tree or a chain; one decoded token is a tree of one) need beside
+ * the MoE layer that runs the same rows (qf_moe.h). No counterpart in the
+ * reference's MoE path: entry points and layouts are this library's own.
+ *
+ * Cache rows are quantised as they are written, per token and head:
+ *   amax = max_d |v[d]|,  s = amax * (1 / 127) (E4M3: amax * (1 / 448)), 1 where that is 0
+ *   INT8 code = rint(v / s) clamped to +-127,  E4M3 code = e4m3(v / s) clamped to +-448
+ *   (fp32 operations, ties to even; the scale by the rule of qf8_i8_x8);  value = code * s
+ * A row that holds a NaN or an infinity is stored as codes 0 with s = NaN: it
+ * reads back as NaN, and a query that sees it gets NaN.
+ *
+ * Conventions as in qf_moe.h: asynchronous, stream-ordered, no allocation, no
+ * host synchronisation, graph-capturable; 0 on success, -1 for a rejected
+ * argument (nothing launched), -3 for a launch error; messages through
+ * qfm_last_error(). Launches go to the current device, where every buffer has
+ * to be. Indices that live in device memory (sequences, positions, pages) are
+ * checked by the kernels, which pass over what is out of range.
+ */
+#ifndef QF_ATTN_H
+#define QF_ATTN_H
+#include "qf_moe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+#pragma GCC visibility push(default)
+
+#define QFM_KV_INT8 0
+#define QFM_KV_E4M3 1
+/* element types of rows */
+#define QFM_DT_F32  0
+#define QFM_DT_BF16 1
+#define QFM_DT_F16  2
+
+/* A layer's pool of pages. page: tokens a page, 16, 32, 64, 128 or 256;
+ * head_dim D: 64, 128 or 256.
+ *   k  codes [n_pages][kv_heads][page][D]
+ *   v  codes [n_pages][kv_heads][page / 4][D][4]: four tokens of one channel
+ *      side by side, so that attention's second product, whose inner dimension
+ *      is the tokens, loads its operand as it lies
+ *   ks, vs  fp32 scales [n_pages][kv_heads][page]
+ * k and v 16-byte aligned. Pages need no initialisation. */
+typedef struct {
+    void  *k, *v;
+    float *ks, *vs;
+    int    n_pages, page, kv_heads, head_dim, fmt;
+} qfm_kv_cache;
+
+/* The sequences' pages: position p of sequence s lies in page
+ * table[s][p / page] (device, int32 [n_seq][max_pages]) at token p % page. A
+ * page id outside [0, n_pages) is no page: rows there are neither written nor
+ * read, and attention does not see them. */
+typedef struct {
+    const int *table;
+    int        n_seq, max_pages;
+} qfm_kv_seqs;
+
+/* T rows of keys and values (k and v: element (t, h, d) at t * row_stride +
+ * h * head_stride + d, type dtype) into positions pos[t] of the sequences
+ * seq[t] (device int32 [T]). Strides are multiples of 8 and not negative, k and
+ * v 16-byte aligned. A row whose sequence, position or page does not exist
+ * (pos -1, say) is passed over. Rows of one call name different places: of two
+ * that name the same one, codes and scale may be from either. */
+int qfm_kv_write(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *k, const void *v, int dtype,
+                 long row_stride, long head_stride, const int *seq, const int *pos, int T, hipStream_t s);
+
+/* The same rows back as values (code * scale, rounded once to dtype) into k
+ * and v, either of which may be NULL. Strides as above and at least D. A row
+ * that does not exist is left as it was. */
+int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, int dtype, long row_stride,
+                long head_stride, const int *seq, const int *pos, int T, hipStream_t s);
+
+#pragma GCC visibility pop
+#ifdef __cplusplus
+}
+#endif
+#endif

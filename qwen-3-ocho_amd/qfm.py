@@ -1,4 +1,4 @@
-"""ctypes binding of libqfm.so (the C ABI declared in include/qf_moe.h).
+"""ctypes binding of libqfm.so (the C ABI declared in include/).
 
 This is the Python side of the boundary used by the tests, the smoke check
 and bench.py: it loads the in-tree HIP library, mirrors its structs and
@@ -15,6 +15,8 @@ LIB_PATH = os.path.join(HERE, "libqfm.so")
 
 QFM_FMT_INT8 = 0
 QFM_FMT_NVFP4 = 1
+QFM_KV_INT8, QFM_KV_E4M3 = 0, 1
+QFM_DT = {"f32": 0, "bf16": 1, "f16": 2}
 GEN_I8, GEN_ROWSCALE, GEN_GAUSS_F32, GEN_GAUSS_BF16, GEN_FP4BYTE, GEN_E4M3SCALE = range(6)
 
 vp = C.c_void_p
@@ -108,6 +110,17 @@ class Qf8ShexpW(C.Structure):
 class Qf8MoeDesc(C.Structure):
     """FP8 path expert descriptor (qf8_moe_fp8.h:37-44)."""
     _fields_ = [("slot", C.c_int), ("nrow", C.c_int), ("row", C.c_int * 16), ("wt", C.c_float * 16)]
+
+
+class QfmKvCache(C.Structure):
+    """A layer's pool of cache pages (qf_attn.h)."""
+    _fields_ = [("k", vp), ("v", vp), ("ks", vp), ("vs", vp), ("n_pages", C.c_int), ("page", C.c_int),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("fmt", C.c_int)]
+
+
+class QfmKvSeqs(C.Structure):
+    """The sequences' page table (qf_attn.h)."""
+    _fields_ = [("table", vp), ("n_seq", C.c_int), ("max_pages", C.c_int)]
 
 
 DTYPE_CODES = {"BF16": 1, "F32": 2, "U8": 3, "F8_E4M3": 4, "I64": 5, "F16": 6, "I8": 7, "I32": 8,
@@ -236,6 +249,10 @@ _SIGS = {
     "qf8_shexp_ex": (C.c_int, [C.POINTER(Qf8ShexpW), vp, vp, vp, vp, vp, vp, vp]),
     "qf8_shexp_M": (None, [C.POINTER(Qf8ShexpW), vp, C.c_int, vp, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
     "qf8_shexp_M_ex": (C.c_int, [C.POINTER(Qf8ShexpW), vp, C.c_int, vp, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
+    "qfm_kv_write": (C.c_int, [C.POINTER(QfmKvCache), C.POINTER(QfmKvSeqs), vp, vp, C.c_int, C.c_long, C.c_long,
+                               vp, vp, C.c_int, vp]),
+    "qfm_kv_read": (C.c_int, [C.POINTER(QfmKvCache), C.POINTER(QfmKvSeqs), vp, vp, C.c_int, C.c_long, C.c_long,
+                              vp, vp, C.c_int, vp]),
     "qfm_gen_input_rows": (C.c_int, [vp, C.c_int, C.c_uint32, C.c_uint32, C.c_int, vp]),
     "qfm_dev_malloc": (vp, [C.c_size_t]),
     "qfm_dev_free": (C.c_int, [vp]),

@@ -1,0 +1,71 @@
+"""What the cache, attention and adapter entry points refuse: every call here is
+rejected on the host, before any launch, so this runs without a GPU."""
+import ctypes as C
+
+import pytest
+
+import qfm
+
+P = 1 << 20                                          # an aligned address that nothing follows
+
+
+@pytest.fixture
+def lib():
+    lib = qfm.load()
+    lib.qfm_last_error()
+    return lib
+
+
+def _cache(**kw):
+    a = dict(k=P, v=P, ks=P, vs=P, n_pages=8, page=16, kv_heads=2, head_dim=128, fmt=0)
+    a.update(kw)
+    return qfm.QfmKvCache(*a.values())
+
+
+def _seqs(**kw):
+    a = dict(table=P, n_seq=2, max_pages=3)
+    a.update(kw)
+    return qfm.QfmKvSeqs(*a.values())
+
+
+BAD_CACHES = [dict(k=None), dict(v=None), dict(ks=None), dict(vs=None), dict(n_pages=0), dict(n_pages=-1), dict(page=8),
+              dict(page=48), dict(page=512), dict(page=0), dict(page=-16), dict(kv_heads=0), dict(kv_heads=1025), dict(head_dim=96),
+              dict(head_dim=512), dict(head_dim=0), dict(fmt=2), dict(fmt=-1), dict(k=P + 8), dict(v=P + 1), dict(ks=P + 4), dict(vs=P + 2)]
+BAD_SEQS = [dict(table=None), dict(n_seq=0), dict(n_seq=65536), dict(max_pages=0)]
+
+
+def _rows_call(lib, name, cache, seqs, **kw):
+    a = dict(k=P, v=P, dtype=1, rs=256, hs=128, seq=P, pos=P, T=4)
+    a.update(kw)
+    rc = getattr(lib, name)(C.byref(cache) if cache else None, C.byref(seqs) if seqs else None, *a.values(), None)
+    return rc, lib.qfm_last_error()
+
+
+@pytest.mark.parametrize("name", ["qfm_kv_write", "qfm_kv_read"])
+def test_rows_refuse(lib, name):
+    for bad in BAD_CACHES:
+        rc, msg = _rows_call(lib, name, _cache(**bad), _seqs())
+        assert rc == -1 and name.encode() in msg, bad
+    for bad in BAD_SEQS:
+        rc, msg = _rows_call(lib, name, _cache(), _seqs(**bad))
+        assert rc == -1 and name.encode() in msg, bad
+    for bad in (dict(dtype=3), dict(dtype=-1), dict(rs=-8), dict(hs=-8), dict(rs=252), dict(hs=129), dict(seq=None),
+                dict(pos=None), dict(T=-1), dict(T=(1 << 24) + 1), dict(k=P + 8), dict(v=P + 2), dict(k=None, v=None)):
+        rc, msg = _rows_call(lib, name, _cache(), _seqs(), **bad)
+        assert rc == -1 and name.encode() in msg, bad
+    for c, s in ((None, _seqs()), (_cache(), None)):
+        assert _rows_call(lib, name, c, s)[0] == -1
+    assert _rows_call(lib, name, _cache(), _seqs(), T=0)[0] == 0      # nothing to do
+
+
+def test_write_needs_both_rows_and_read_rows_apart(lib):
+    assert _rows_call(lib, "qfm_kv_write", _cache(), _seqs(), k=None)[0] == -1
+    assert _rows_call(lib, "qfm_kv_write", _cache(), _seqs(), v=None)[0] == -1
+    # results that would lie on each other
+    assert _rows_call(lib, "qfm_kv_read", _cache(), _seqs(), rs=0)[0] == -1
+    assert _rows_call(lib, "qfm_kv_read", _cache(), _seqs(), hs=120)[0] == -1
+
+
+def test_struct_layouts():
+    assert C.sizeof(qfm.QfmKvCache) == 56 and qfm.QfmKvCache.fmt.offset == 48
+    assert C.sizeof(qfm.QfmKvSeqs) == 16
