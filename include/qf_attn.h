@@ -73,6 +73,36 @@ int qfm_kv_write(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *k, co
 int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, int dtype, long row_stride,
                 long head_stride, const int *seq, const int *pos, int T, hipStream_t s);
 
+/* Attention of the newest rows of every sequence over its cached keys and
+ * values. Sequence s has the rows row_start[s] .. row_start[s + 1] - 1 of q
+ * (device int32 [n_seq + 1], ascending, at most max_nodes <= 64 a sequence) and
+ * ctx[s] tokens before them; its row i, node i of a tree of drafted tokens,
+ * lies at position ctx[s] + i of the cache, written there before this call.
+ * Row i sees every position below ctx[s], and node j of its own sequence where
+ * bit j of tree[row_start[s] + i] is set (its ancestors and, as a rule, itself);
+ * tree NULL: the nodes are a chain, row i sees nodes 0..i. One decoded token
+ * is max_nodes 1, its mask 1 or NULL.
+ *   out(t, h) = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q(t, h) . k_j - max)
+ * over the positions that row t sees, with the keys and values of head
+ * h / (q_heads / kv_heads). A row that sees nothing gets zeros. Scores, maxima,
+ * sums and results are held in fp32; q and p enter the products as fp16 scaled
+ * by powers of two (F32 rows: as two fp16 numbers, 22 bits), the codes exactly.
+ *   q, out  element (t, h, d) at t * row_stride + h * head_stride + d, type
+ *           dtype; strides multiples of 8 and not negative (out: at least D),
+ *           16-byte aligned. Rows of out that no sequence has are left.
+ *   T       rows of q; row_start beyond it is cut there
+ *   max_ctx the largest ctx the host expects: it sets how far a sequence's keys
+ *           are split over the GPU, nothing else (longer ones are right, too)
+ *   scale   > 0
+ *   ws      at least qfm_tree_attn_ws_bytes of the same arguments, 16-byte
+ *           aligned, no initialisation; calls that share it must not overlap.
+ *           0 bytes: ws may be NULL. */
+size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx);
+int    qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, void *out, int dtype, int q_heads,
+                     long q_row_stride, long q_head_stride, long out_row_stride, long out_head_stride,
+                     const int *row_start, const int *ctx, const uint64_t *tree, int T, int max_nodes, int max_ctx,
+                     float scale, void *ws, size_t ws_bytes, hipStream_t s);
+
 #pragma GCC visibility pop
 #ifdef __cplusplus
 }

@@ -1,0 +1,481 @@
+// qfm_attn.hip -- attention of drafted rows over the quantised cache
+// (qfm_tree_attn).
+//
+// One workgroup of four waves takes up to 16 RB rows (nodes x the query heads
+// that share a key/value head) and a range of 32-token tiles; the waves take
+// the tiles in turn, each with a running maximum, sum and result of its own,
+// joined through LDS at the end and, where a sequence's keys are split over
+// workgroups, once more by k_tree_join. No wave waits for another inside the
+// loop, and every cached byte enters the registers of one wave only, straight
+// from memory:
+//   S^T = K Q^T   the MFMA's rows are tokens. A lane's 16 bytes of a key row
+//                 (d = 64 c + 16 g + 0..15, g = lane / 16) are two k-steps; Q is
+//                 laid out to match.
+//   O^T = V^T P^T lane (g, r) of S^T holds tokens 4 g + i of both 16-token halves
+//                 for row r, which is the layout the second product wants of
+//                 P^T when its inner index runs over (half, 4 g + i) in that
+//                 order: no exchange between lanes. V's layout (four tokens of
+//                 a channel side by side) gives a lane the same tokens of 4
+//                 channels in 16 bytes.
+// Codes are widened to fp16 exactly (int8 and E4M3 both fit); a row of Q is
+// scaled to [2^14, 2^15) by a power of two; p times the value's scale is kept
+// within fp16 by a power of two of the largest value scale so far. F32 rows
+// carry Q and P as two fp16 numbers each and take every product twice.
+#include "qfm_kv.h"
+#include "qfm_mfma.h"
+#include "qfm_internal.h"
+
+namespace qfm {
+
+constexpr int kAttnWaves = 4;
+constexpr float kNoMax = -3.402823466e38f;
+constexpr float kLazy = 8.0f;      // the maximum may be exceeded by 2^8 before sums and results are rescaled
+constexpr int kVeMin = -118;       // least exponent of the value scale that the products are kept relative to
+
+struct AttnArgs {
+    const uint8_t *q;
+    uint8_t *out;
+    int dtype, G, T, max_nodes, splits;
+    long qrs, qhs, ors, ohs;
+    const int *row_start, *ctx;
+    const uint64_t *tree;
+    float scale;
+    float *po;                     // [splits][T][q_heads][D], normalised
+    float2 *pml;                   // [splits][T][q_heads] {maximum (base 2), sum}
+};
+
+// the rows of sequence s: first row, count
+__device__ __forceinline__ int2 seq_rows(const int *row_start, int s, int T, int max_nodes) {
+    const int r0 = row_start[s], r1 = min(row_start[s + 1], T);
+    return make_int2(r0, r0 < 0 || r1 <= r0 ? 0 : min(r1 - r0, max_nodes));
+}
+
+template <int FMT>
+__device__ __forceinline__ void codes16(u32x4_t w, f16x8_t &a, f16x8_t &b) {
+    if constexpr (FMT == QFM_KV_INT8) {
+        i8_to_f16(w, a, b);
+    } else {
+        uint32_t o[8];
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            o[2 * q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[q], 1.0f, 0));
+            o[2 * q + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[q], 1.0f, 1));
+        }
+        a = __builtin_bit_cast(f16x8_t, u32x4_t{o[0], o[1], o[2], o[3]});
+        b = __builtin_bit_cast(f16x8_t, u32x4_t{o[4], o[5], o[6], o[7]});
+    }
+}
+
+__device__ __forceinline__ float max_over_g(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float sum_over_g(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+__device__ __forceinline__ float pow2_ratio(int d) { return d < -126 ? 0.0f : exp2i(min(d, 127)); }
+
+// 4 values rounded to dtype
+__device__ __forceinline__ void store4(uint8_t *out, long at, int dtype, float4 v) {
+    if (dtype == QFM_DT_F32) *reinterpret_cast<float4 *>(out + at * 4) = v;
+    else if (dtype == QFM_DT_BF16)
+        *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_BF16>(v.x, v.y), pack2<QFM_DT_BF16>(v.z, v.w));
+    else *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_F16>(v.x, v.y), pack2<QFM_DT_F16>(v.z, v.w));
+}
+
+template <int FMT, int D, int RB, bool F32>
+__global__ void __launch_bounds__(64 * kAttnWaves)
+k_tree_attn(KvView c, AttnArgs a) {
+    constexpr int NC = D / 64, NP = F32 ? 2 : 1, ROWS = 16 * RB, LD = D + 4;
+    __shared__ float s_o[kAttnWaves][ROWS * LD];
+    __shared__ float s_m[kAttnWaves][ROWS], s_l[kAttnWaves][ROWS];
+    __shared__ int s_ve[kAttnWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+    const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
+    const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
+    const int rows = sr.y * a.G, row0 = blk * ROWS;
+    if (row0 >= rows) return;
+    const long cap = (long)c.max_pages << c.page_log2;
+    const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
+    const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
+    const int t1 = min(nt, ((int)blockIdx.x + 1) * per);
+
+    // Q: fp16 fragments scaled per row, and what undoes the scaling
+    f16x8_t qf[RB][NC][2][NP];
+    float qs[RB];
+    uint64_t see[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        const int r = row0 + 16 * rb + l16, rr = min(r, rows - 1), node = rr / a.G;
+        const uint8_t *p = a.q + ((sr.x + node) * a.qrs + (long)(h * a.G + rr - node * a.G) * a.qhs) * (F32 ? 4 : 2);
+        float v[NC][2][8], m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const uint8_t *at = p + (64 * k + 16 * g + 8 * j) * (F32 ? 4 : 2);
+                if constexpr (F32) load8<QFM_DT_F32>(at, v[k][j]);
+                else if (a.dtype == QFM_DT_BF16) load8<QFM_DT_BF16>(at, v[k][j]);
+                else load8<QFM_DT_F16>(at, v[k][j]);
+#pragma unroll
+                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
+            }
+        const int k2 = f16_exp(max_over_g(m));
+        const float sc = exp2i(k2);
+        qs[rb] = exp2i(-k2) * (a.scale * 1.4426950408889634f);
+        see[rb] = a.tree ? a.tree[sr.x + node] : node == 63 ? ~0ull : (2ull << node) - 1;
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = v[k][j][e] * sc;
+                    const _Float16 hi = (_Float16)x;
+                    qf[rb][k][j][0][e] = hi;
+                    if constexpr (F32) qf[rb][k][j][NP - 1][e] = (_Float16)(x - (float)hi);
+                }
+    }
+
+    f32x4_t o[RB][NC][4];
+    float m[RB], l[RB];
+    int ve = kVeMin;
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        m[rb] = kNoMax;
+        l[rb] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int t = 0; t < 4; t++) o[rb][k][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int t = (int)blockIdx.x * per + wave; t < t1; t += kAttnWaves) {
+        int page[2];
+        u32x4_t kr[2][NC], vr[2][NC];
+        float ks[2][4], vs[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int p = 32 * t + 16 * i;
+            page[i] = p < len ? c.page_of(seq, p) : -1;
+            const size_t at = c.token0(max(page[i], 0), h) + (p & (c.page() - 1));
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                kr[i][k] = *reinterpret_cast<const u32x4_t *>(c.k + (at + l16) * D + 64 * k + 16 * g);
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                vr[i][k] = *reinterpret_cast<const u32x4_t *>(c.v + (at + 4 * g) * D + (64 * k + 4 * l16) * 4);
+            const float4 x = *reinterpret_cast<const float4 *>(c.ks + at + 4 * g);
+            const float4 y = *reinterpret_cast<const float4 *>(c.vs + at + 4 * g);
+            ks[i][0] = x.x; ks[i][1] = x.y; ks[i][2] = x.z; ks[i][3] = x.w;
+            vs[i][0] = y.x; vs[i][1] = y.y; vs[i][2] = y.z; vs[i][3] = y.w;
+        }
+        // scores
+        f32x4_t s[RB][2];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) s[rb][0] = s[rb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int k = 0; k < NC; k++) {
+                f16x8_t ka, kb;
+                codes16<FMT>(kr[i][k], ka, kb);
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int n = 0; n < NP; n++) {
+                        s[rb][i] = mfma_f16(ka, qf[rb][k][0][n], s[rb][i]);
+                        s[rb][i] = mfma_f16(kb, qf[rb][k][1][n], s[rb][i]);
+                    }
+            }
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[i][e] * qs[rb];
+        const bool edge = 32 * t + 32 > ctx || page[0] < 0 || page[1] < 0;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int j0 = 32 * t + 16 * i + 4 * g, n = page[i] < 0 ? 0 : min(max(len - j0, 0), 4);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (e >= n) vs[i][e] = 0.0f;
+#pragma unroll
+                    for (int rb = 0; rb < RB; rb++) {
+                        const int j = j0 + e - ctx;
+                        if (e >= n || (j >= 0 && !(see[rb] >> j & 1))) s[rb][i][e] = -INFINITY;
+                    }
+                }
+                if constexpr (FMT == QFM_KV_E4M3) {       // a NaN code times 0 would be NaN
+                    const uint32_t keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+                    for (int k = 0; k < NC; k++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) vr[i][k][q] &= keep;
+                }
+            }
+        }
+        // the largest score so far, and the largest value scale
+        bool grow = false;
+        float top[RB], vm = 0.0f;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            top[rb] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top[rb] = fmaxf(top[rb], s[rb][i][e]);
+            grow |= top[rb] > m[rb] + kLazy;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vm = fmaxf(vm, vs[i][e]);
+        grow |= vm >= exp2i(ve) * 2.0f;
+        if (__any(grow)) {
+            const int vn = max(ve, (int)(__float_as_uint(max_over_g(vm)) >> 23) - 127);
+            const float vf = pow2_ratio(ve - vn);
+            ve = vn;
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) {
+                const float mn = fmaxf(m[rb], max_over_g(top[rb])), f = exp2f(m[rb] - mn);
+                m[rb] = mn;
+                l[rb] *= f;
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) o[rb][k][q] *= f * vf;
+            }
+        }
+        const float vi = exp2i(6 - ve);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vs[i][e] *= vi;
+        f16x8_t pf[RB][NP];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = exp2f(s[rb][i][e] - m[rb]);
+                    l[rb] += p;
+                    float x = p * vs[i][e];
+                    if (edge && s[rb][i][e] == -INFINITY) x = 0.0f;   // not seen: its scale may be NaN
+                    const _Float16 hi = (_Float16)x;
+                    pf[rb][0][4 * i + e] = hi;
+                    if constexpr (F32) pf[rb][NP - 1][4 * i + e] = (_Float16)(x - (float)hi);
+                }
+        // results
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            f16x8_t a0, b0, a1, b1;
+            codes16<FMT>(vr[0][k], a0, b0);
+            codes16<FMT>(vr[1][k], a1, b1);
+            const f16x8_t vf[4] = {__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 8, 9, 10, 11),
+                                   __builtin_shufflevector(a0, a1, 4, 5, 6, 7, 12, 13, 14, 15),
+                                   __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 8, 9, 10, 11),
+                                   __builtin_shufflevector(b0, b1, 4, 5, 6, 7, 12, 13, 14, 15)};
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int n = 0; n < NP; n++) o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], o[rb][k][q]);
+        }
+    }
+
+    // join the waves
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        l[rb] = sum_over_g(l[rb]);
+        if (g == 0) {
+            s_m[wave][16 * rb + l16] = m[rb];
+            s_l[wave][16 * rb + l16] = l[rb];
+        }
+    }
+    if (lane == 0) s_ve[wave] = ve;
+    __syncthreads();
+    int vn = s_ve[0];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; w++) vn = max(vn, s_ve[w]);
+    const float vf = pow2_ratio(ve - vn);
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        float mn = s_m[0][16 * rb + l16];
+#pragma unroll
+        for (int w = 1; w < kAttnWaves; w++) mn = fmaxf(mn, s_m[w][16 * rb + l16]);
+        const float f = exp2f(m[rb] - mn) * vf;
+        // channel 64 k + 16 g + 4 i + q of row l16: element i of o[rb][k][q]
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4 *>(&s_o[wave][(16 * rb + l16) * LD + 64 * k + 16 * g + 4 * i]) =
+                    make_float4(o[rb][k][0][i] * f, o[rb][k][1][i] * f, o[rb][k][2][i] * f, o[rb][k][3][i] * f);
+    }
+    __syncthreads();
+    const float back = exp2i(vn - 6);
+    const int heads = c.heads * a.G;
+    for (int e = threadIdx.x; e < ROWS * (D / 4); e += 64 * kAttnWaves) {
+        const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+        if (row0 + r >= rows) break;
+        float mn = s_m[0][r], sum = 0.0f;
+#pragma unroll
+        for (int w = 1; w < kAttnWaves; w++) mn = fmaxf(mn, s_m[w][r]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kAttnWaves; w++) {
+            const float4 y = *reinterpret_cast<const float4 *>(&s_o[w][r * LD + d]);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+            sum += s_l[w][r] * exp2f(s_m[w][r] - mn);
+        }
+        const float inv = sum == 0.0f ? 0.0f : back / sum;
+        x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
+        const int node = (row0 + r) / a.G, head = h * a.G + (row0 + r) - node * a.G;
+        const long t = sr.x + node;
+        if (a.splits == 1) {
+            store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, x);
+        } else {
+            const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
+            *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
+            if (d == 0) a.pml[at] = make_float2(mn, sum);
+        }
+    }
+}
+
+// out(t, h) = sum_s w_s o_s / sum_s w_s, w_s = sum_s 2^(max_s - max): 256 / (D / 4)
+// heads a block.
+template <int D>
+__global__ void __launch_bounds__(256)
+k_tree_join(AttnArgs a, int heads) {
+    const int2 sr = seq_rows(a.row_start, (int)blockIdx.z, a.T, a.max_nodes);
+    const int head = (int)blockIdx.x * (1024 / D) + (int)threadIdx.x / (D / 4), d = (int)threadIdx.x % (D / 4) * 4;
+    if ((int)blockIdx.y >= sr.y || head >= heads) return;
+    const long t = sr.x + (int)blockIdx.y;
+    float mn = kNoMax, sum = 0.0f;
+    for (int s = 0; s < a.splits; s++) mn = fmaxf(mn, a.pml[((size_t)s * a.T + t) * heads + head].x);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.splits; s++) {
+        const size_t at = ((size_t)s * a.T + t) * heads + head;
+        const float2 ml = a.pml[at];
+        const float4 y = *reinterpret_cast<const float4 *>(a.po + at * D + d);
+        const float w = ml.y * exp2f(ml.x - mn);
+        if (ml.y == 0.0f) continue;
+        sum += w;
+        x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+}
+
+// 16-row blocks a workgroup takes: as many as the rows fill, within the
+// registers (64 results a lane and 64 channels of 16 rows)
+static int row_blocks(int D, int rows) { return rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4; }
+
+// workgroups that share a sequence's keys: enough for the GPU's 256 CUs, each
+// with a tile or more for every wave
+static int attn_splits(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx) {
+    const int rows = max_nodes * (q_heads / kv_heads), per = 16 * row_blocks(D, rows);
+    const long groups = (long)n_seq * kv_heads * ((rows + per - 1) / per);
+    const long tiles = ((long)max_ctx + max_nodes + 31) / 32;
+    return (int)max(1l, min((long)min(128l, (768 + groups - 1) / groups), (tiles + kAttnWaves - 1) / kAttnWaves));
+}
+
+static int attn_shape(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
+    if (!c || (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) || c->kv_heads < 1 || c->kv_heads > 1024 ||
+        n_seq < 1 || n_seq > 65535 || T < 0 || T > 1 << 22 || q_heads < 1 || q_heads > 4096 || q_heads % c->kv_heads ||
+        max_nodes < 1 || max_nodes > 64 || max_ctx < 0)
+        return -1;
+    return (long)c->kv_heads * ((max_nodes * (q_heads / c->kv_heads) + 15) / 16) > 65535 ? -1 : 0;
+}
+
+static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
+    return splits == 1 ? 0 : (size_t)splits * T * q_heads * (c->head_dim + 2) * 4;
+}
+
+template <int FMT, int D, int RB>
+static void attn_launch(const KvView &v, const AttnArgs &a, dim3 g, hipStream_t s) {
+    if (a.dtype == QFM_DT_F32) hipLaunchKernelGGL((k_tree_attn<FMT, D, RB, true>), g, dim3(64 * kAttnWaves), 0, s, v, a);
+    else hipLaunchKernelGGL((k_tree_attn<FMT, D, RB, false>), g, dim3(64 * kAttnWaves), 0, s, v, a);
+}
+template <int FMT, int D>
+static void attn_launch(const KvView &v, const AttnArgs &a, int rb, dim3 g, hipStream_t s) {
+    if (rb == 1) attn_launch<FMT, D, 1>(v, a, g, s);
+    else if (rb == 2) attn_launch<FMT, D, 2>(v, a, g, s);
+    else if constexpr (D != 256) attn_launch<FMT, D, 4>(v, a, g, s);
+}
+
+}  // namespace qfm
+
+using namespace qfm;
+
+extern "C" {
+
+size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
+    if (attn_shape(c, n_seq, T, q_heads, max_nodes, max_ctx)) return 0;
+    return attn_ws(c, attn_splits(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx), T, q_heads);
+}
+
+int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, void *out, int dtype, int q_heads,
+                  long q_row_stride, long q_head_stride, long out_row_stride, long out_head_stride, const int *row_start,
+                  const int *ctx, const uint64_t *tree, int T, int max_nodes, int max_ctx, float scale, void *ws,
+                  size_t ws_bytes, hipStream_t s) {
+    const char *who = "qfm_tree_attn";
+    KvView v;
+    if (kv_view(c, sq, &v, who)) return -1;
+    if (attn_shape(c, sq->n_seq, T, q_heads, max_nodes, max_ctx)) {
+        set_error(-1, "%s: T = %d, %d query heads over %d, %d nodes (1..64), max_ctx %d", who, T, q_heads, c->kv_heads,
+                  max_nodes, max_ctx);
+        return -1;
+    }
+    if (dtype != QFM_DT_F32 && dtype != QFM_DT_BF16 && dtype != QFM_DT_F16) {
+        set_error(-1, "%s: element type %d", who, dtype);
+        return -1;
+    }
+    if (!q || !out || !row_start || !ctx) { set_error(-1, "%s: null argument", who); return -1; }
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15 || reinterpret_cast<uintptr_t>(tree) & 7) {
+        set_error(-1, "%s: q and out are 16-byte aligned, the masks 8", who);
+        return -1;
+    }
+    if (q_row_stride < 0 || q_head_stride < 0 || q_row_stride % 8 || q_head_stride % 8 || out_row_stride % 8 ||
+        out_head_stride % 8 || out_row_stride < c->head_dim || out_head_stride < c->head_dim) {
+        set_error(-1, "%s: strides %ld %ld %ld %ld (multiples of 8, those of out at least %d)", who, q_row_stride,
+                  q_head_stride, out_row_stride, out_head_stride, c->head_dim);
+        return -1;
+    }
+    if (!(scale > 0.0f) || !(scale < 3.4e38f)) { set_error(-1, "%s: scale %g", who, (double)scale); return -1; }
+    const int D = c->head_dim, G = q_heads / c->kv_heads, rb = row_blocks(D, max_nodes * G);
+    const int splits = attn_splits(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx);
+    const size_t need = attn_ws(c, splits, T, q_heads);
+    if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) & 15)) {
+        set_error(-1, "%s: workspace of %zu bytes (16-byte aligned), %zu needed", who, ws ? ws_bytes : (size_t)0, need);
+        return -1;
+    }
+    if (T == 0) return 0;
+    AttnArgs a{static_cast<const uint8_t *>(q), static_cast<uint8_t *>(out), dtype, G, T, max_nodes, splits,
+               q_row_stride, q_head_stride, out_row_stride, out_head_stride, row_start, ctx, tree, scale, nullptr, nullptr};
+    a.po = static_cast<float *>(ws);
+    if (splits > 1) a.pml = reinterpret_cast<float2 *>(a.po + (size_t)splits * T * q_heads * D);
+    const dim3 g((unsigned)splits, (unsigned)(c->kv_heads * ((max_nodes * G + 16 * rb - 1) / (16 * rb))), (unsigned)sq->n_seq);
+    const bool i8 = c->fmt == QFM_KV_INT8;
+    switch (D) {
+        case 64: i8 ? attn_launch<QFM_KV_INT8, 64>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 64>(v, a, rb, g, s); break;
+        case 128: i8 ? attn_launch<QFM_KV_INT8, 128>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 128>(v, a, rb, g, s); break;
+        default: i8 ? attn_launch<QFM_KV_INT8, 256>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 256>(v, a, rb, g, s); break;
+    }
+    if (check_launch(who)) return -3;
+    if (splits > 1) {
+        const dim3 gj((unsigned)((q_heads + 1024 / D - 1) / (1024 / D)), (unsigned)max_nodes, (unsigned)sq->n_seq);
+        if (D == 64) hipLaunchKernelGGL(k_tree_join<64>, gj, dim3(256), 0, s, a, q_heads);
+        else if (D == 128) hipLaunchKernelGGL(k_tree_join<128>, gj, dim3(256), 0, s, a, q_heads);
+        else hipLaunchKernelGGL(k_tree_join<256>, gj, dim3(256), 0, s, a, q_heads);
+    }
+    return check_launch(who) ? -3 : 0;
+}
+
+}  // extern "C"

@@ -253,6 +253,9 @@ _SIGS = {
                                vp, vp, C.c_int, vp]),
     "qfm_kv_read": (C.c_int, [C.POINTER(QfmKvCache), C.POINTER(QfmKvSeqs), vp, vp, C.c_int, C.c_long, C.c_long,
                               vp, vp, C.c_int, vp]),
+    "qfm_tree_attn_ws_bytes": (C.c_size_t, [C.POINTER(QfmKvCache)] + [C.c_int] * 5),
+    "qfm_tree_attn": (C.c_int, [C.POINTER(QfmKvCache), C.POINTER(QfmKvSeqs), vp, vp, C.c_int, C.c_int] + [C.c_long] * 4 +
+                      [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, vp, C.c_size_t, vp]),
     "qfm_gen_input_rows": (C.c_int, [vp, C.c_int, C.c_uint32, C.c_uint32, C.c_int, vp]),
     "qfm_dev_malloc": (vp, [C.c_size_t]),
     "qfm_dev_free": (C.c_int, [vp]),

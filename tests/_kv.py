@@ -149,3 +149,83 @@ def scatter(a, n, rs, hs, fill=0):
     at = np.arange(T)[:, None, None] * rs + np.arange(H)[None, :, None] * hs + np.arange(D)
     out[at.ravel()] = a.ravel()
     return out, at
+
+
+# ---- attention ----------------------------------------------------------------------
+def fill_rows(c, s, n, rng, spread=0.5):
+    """Positions 0..n-1 of sequence s: codes and scales as a writer leaves them (pages that exist only)."""
+    pos = np.arange(n)
+    inside = pos // c.page < c.table.shape[1]
+    pos = pos[inside]
+    g = c.table[s, pos // c.page]
+    ok = (g >= 0) & (g < c.pages)
+    g, o = g[ok], pos[ok] % c.page
+    for name, sc in (("k", "ks"), ("v", "vs")):
+        x = rng.standard_normal((len(g), c.heads, c.dim)).astype(np.float32)
+        x *= np.exp(rng.normal(0, spread, (len(g), c.heads, 1))).astype(np.float32)
+        code, scale = quantise(x, c.fmt)
+        if name == "k":
+            c.k[g, :, o] = code
+        else:
+            c.v[g, :, o // 4, :, o % 4] = code
+        getattr(c, sc)[g, :, o] = scale
+
+
+def tree_masks(counts, rng):
+    """Masks of random trees, a node's ancestors and itself, [sum counts] uint64."""
+    out = []
+    for m in counts:
+        t = []
+        for j in range(m):
+            up = int(rng.integers(-1, j)) if j else -1
+            t.append((t[up] if up >= 0 else 0) | 1 << j)
+        out += t
+    return np.array(out, np.uint64)
+
+
+def attention(c, q, row_start, ctx, tree, scale, dt):
+    """(out, tolerance) in 64 bits, [T][q_heads][dim]; the tolerance of rows that no sequence has is -1.
+
+    The tolerance, element by element, with A = sum p |v| / sum p and u = 2^-24:
+      the result's own rounding, EPS[dt] |out|;
+      p times the value scale in fp16 (2^-11 relative; two numbers, 2^-22, for f32), and below fp16's normal range
+      half a step of 2^-24, where the largest value scale is kept at 2^6: 2^-24 of it a position at most;
+      scores: a sum of D products in fp32, 6 sqrt(D) u sum |q k| (roundings that are independent pass it once in
+      1e7), q as two fp16 numbers 2^-22 of it for f32, three more roundings of the scaled score and one of its
+      exponent: relative errors of p, twice (numerator and sum);
+      the sums over n positions in fp32, 6 sqrt(n) u each, and the joins of up to 4 waves and 128 splits, 10
+      roundings each.
+    """
+    T, Hq, D = q.shape
+    G, u = Hq // c.heads, 2.0 ** -24
+    out, tol = np.full(q.shape, np.nan), np.full(q.shape, -1.0)
+    val, q = CODE_VALUE[c.fmt], q.astype(np.float64)
+    cap = c.table.shape[1] * c.page
+    for s in range(len(ctx)):
+        r0, r1 = int(row_start[s]), min(int(row_start[s + 1]), T)
+        m, cx = max(r1 - r0, 0), min(max(int(ctx[s]), 0), cap)
+        pos = np.arange(min(cx + m, cap))
+        g = c.table[s, pos // c.page]
+        ok = (g >= 0) & (g < c.pages)
+        pos, g = pos[ok], g[ok]
+        o = pos % c.page
+        k = val[c.k[g, :, o]] * c.ks[g, :, o].astype(np.float64)[..., None]
+        v = val[c.v[g, :, o // 4, :, o % 4]] * c.vs[g, :, o].astype(np.float64)[..., None]
+        for i in range(m):
+            bits = int(tree[r0 + i]) if tree is not None else (2 << i) - 1
+            see = np.array([p < cx or bool(bits >> int(p - cx) & 1) for p in pos], bool)
+            for h in range(Hq):
+                kk, vv, n = k[see, h // G], v[see, h // G], int(see.sum())
+                if not n:
+                    out[r0 + i, h], tol[r0 + i, h] = 0.0, 0.0
+                    continue
+                x = kk @ q[r0 + i, h] * scale
+                p = np.exp(x - x.max())
+                a = p @ np.abs(vv) / p.sum()
+                out[r0 + i, h] = p @ vv / p.sum()
+                mag = (np.abs(kk) @ np.abs(q[r0 + i, h])).max() * scale
+                eq, ep = (2.0 ** -22, 2.0 ** -22) if dt == "f32" else (0.0, 2.0 ** -11)
+                dx = mag * (6 * D ** 0.5 * u + eq) + (np.abs(x).max() + 1) * 4 * u
+                tol[r0 + i, h] = (EPS[dt] * np.abs(out[r0 + i, h]) + a * (ep + 2 * dx + (12 * n ** 0.5 + 20) * u) +
+                                  n * 2.0 ** -24 * c.vs[g][:, h // G].max(initial=0, where=np.isfinite(c.vs[g][:, h // G])))
+    return out, tol

@@ -69,3 +69,39 @@ def test_write_needs_both_rows_and_read_rows_apart(lib):
 def test_struct_layouts():
     assert C.sizeof(qfm.QfmKvCache) == 56 and qfm.QfmKvCache.fmt.offset == 48
     assert C.sizeof(qfm.QfmKvSeqs) == 16
+
+
+def _attn_call(lib, cache=None, seqs=None, **kw):
+    a = dict(q=P, out=P, dtype=1, q_heads=8, qrs=1024, qhs=128, ors=1024, ohs=128, start=P, ctx=P, tree=P, T=4, nodes=2,
+             max_ctx=100, scale=0.1, ws=P, wsb=1 << 40)
+    a.update(kw)
+    rc = lib.qfm_tree_attn(C.byref(cache or _cache()), C.byref(seqs or _seqs()), *a.values(), None)
+    return rc, lib.qfm_last_error()
+
+
+def test_attention_refuses(lib):
+    for bad in BAD_CACHES:
+        rc, msg = _attn_call(lib, _cache(**bad))
+        assert rc == -1 and b"qfm_tree_attn" in msg, bad
+    for bad in BAD_SEQS:
+        rc, msg = _attn_call(lib, seqs=_seqs(**bad))
+        assert rc == -1 and b"qfm_tree_attn" in msg, bad
+    for bad in (dict(q=None), dict(out=None), dict(start=None), dict(ctx=None), dict(q=P + 8), dict(out=P + 2), dict(tree=P + 4),
+                dict(dtype=3), dict(q_heads=0), dict(q_heads=7), dict(q_heads=4098), dict(qrs=-8), dict(qhs=4), dict(ors=120),
+                dict(ohs=0), dict(ohs=129), dict(T=-1), dict(T=(1 << 22) + 1), dict(nodes=0), dict(nodes=65), dict(max_ctx=-1),
+                dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
+        rc, msg = _attn_call(lib, **bad)
+        assert rc == -1 and b"qfm_tree_attn" in msg, bad
+    assert _attn_call(lib, T=0)[0] == 0
+
+
+def test_attention_asks_for_its_workspace(lib):
+    c = _cache()
+    need = lib.qfm_tree_attn_ws_bytes(C.byref(c), 2, 4, 8, 2, 8000)
+    assert need > 0 and lib.qfm_tree_attn_ws_bytes(C.byref(c), 2, 4, 8, 2, 0) == 0
+    for bad in (dict(ws=None), dict(wsb=need - 1), dict(ws=P + 8), dict(wsb=0)):
+        rc, msg = _attn_call(lib, max_ctx=8000, **bad)
+        assert rc == -1 and b"workspace" in msg, bad
+    for args in ((0, 4, 8, 2, 10), (2, -1, 8, 2, 10), (2, 4, 7, 2, 10), (2, 4, 8, 65, 10), (2, 4, 8, 0, 10), (2, 4, 8, 2, -1)):
+        assert lib.qfm_tree_attn_ws_bytes(C.byref(c), *args) == 0
+    assert lib.qfm_tree_attn_ws_bytes(None, 2, 4, 8, 2, 10) == 0
