@@ -32,6 +32,37 @@ void qf8_i8_gemv_multi(const Qf8I8Multi *mm, const int8_t *xq, const float *xs, 
  * qf8_i8_gemv_rows (qf8_dense_i8.h:35, qf8_dense_i8.hip:252-263). */
 int  qf8_i8_gemv_rows(const Qf8I8Multi *mm, const int8_t *xq, const float *xs, int T, hipStream_t s);
 
+/* Low-rank adapters of many requests beside up to 4 projections that all rows
+ * share (those of qf8_i8_gemv_rows, say, whose y can be base and y here). Slots
+ * hold the adapters as an arena does: slot e has a[i] [slots][R][K], b[i]
+ * [slots][rows[i]][R] (16-bit elements of type dtype, QFM_DT_BF16 or QFM_DT_F16
+ * of qf_attn.h), of which the first rank[e] rows of a and columns of b count
+ * (device int32 [slots], clamped to 0..R; the others may hold anything), and a
+ * factor scale[e] (device fp32 [slots]):
+ *   y[i][t] = base[i][t] + scale[e] * b[i][e] (a[i][e] x[t]),   e = slot[t]
+ * for T rows x [T] at x_stride elements (type dtype) and slot [T] (device
+ * int32); a row whose slot is not in [0, slots) has no adapter: y = base. base[i]
+ * and y[i] are fp32 [T][rows[i]]; base[i] may be y[i] (added in place) or NULL
+ * (zeros). The inner row a x is held in fp32 and enters the second product
+ * whole (three bf16 numbers, or two fp16 ones scaled by a power of two).
+ * 1 <= n <= 4; K a multiple of 64 up to 65536; R a multiple of 8 up to 128;
+ * T up to 2^20; x, a, b, base and y 16-byte aligned, x_stride a multiple of 8
+ * and not negative. No counterpart in the reference. */
+typedef struct {
+    const void  *a[4], *b[4];
+    const float *base[4];
+    float       *y[4];
+    const int   *rank;
+    const float *scale;
+    int          rows[4];
+    int          n, K, R, slots, dtype;
+} qfm_lora;
+/* ws: qfm_lora_ws_bytes(l, T) bytes, 16-byte aligned, no initialisation; calls
+ * that share it must not overlap. 0, -1 (nothing launched) or -3. */
+size_t qfm_lora_ws_bytes(const qfm_lora *l, int T);
+int    qfm_lora_rows(const qfm_lora *l, const void *x, long x_stride, const int *slot, int T, void *ws,
+                     size_t ws_bytes, hipStream_t s);
+
 /* FFN-side hyper-connection pre-mixer, one row (qf8_dense_i8.h:47-58,
  * qf8_dense_i8.hip:109-175, :360-375):
  *   (optional) R[c] += inj_prev[c] * y_prev          (previous mixer's inject, fused)

@@ -123,6 +123,13 @@ class QfmKvSeqs(C.Structure):
     _fields_ = [("table", vp), ("n_seq", C.c_int), ("max_pages", C.c_int)]
 
 
+class QfmLora(C.Structure):
+    """Low-rank adapters beside up to 4 projections (qf_dense.h)."""
+    _fields_ = [("a", vp * 4), ("b", vp * 4), ("base", vp * 4), ("y", vp * 4), ("rank", vp), ("scale", vp),
+                ("rows", C.c_int * 4), ("n", C.c_int), ("K", C.c_int), ("R", C.c_int), ("slots", C.c_int),
+                ("dtype", C.c_int)]
+
+
 DTYPE_CODES = {"BF16": 1, "F32": 2, "U8": 3, "F8_E4M3": 4, "I64": 5, "F16": 6, "I8": 7, "I32": 8,
                "F64": 9, "F8_E5M2": 10, "I16": 11, "U16": 12, "U32": 13, "U64": 14, "BOOL": 15}
 EXPCACHE_NVFP4, EXPCACHE_INT8, EXPCACHE_INT8_ONLY, EXPCACHE_FP8 = 1, 2, 4, 8
@@ -256,6 +263,8 @@ _SIGS = {
     "qfm_tree_attn_ws_bytes": (C.c_size_t, [C.POINTER(QfmKvCache)] + [C.c_int] * 5),
     "qfm_tree_attn": (C.c_int, [C.POINTER(QfmKvCache), C.POINTER(QfmKvSeqs), vp, vp, C.c_int, C.c_int] + [C.c_long] * 4 +
                       [vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, vp, C.c_size_t, vp]),
+    "qfm_lora_ws_bytes": (C.c_size_t, [C.POINTER(QfmLora), C.c_int]),
+    "qfm_lora_rows": (C.c_int, [C.POINTER(QfmLora), vp, C.c_long, vp, C.c_int, vp, C.c_size_t, vp]),
     "qfm_gen_input_rows": (C.c_int, [vp, C.c_int, C.c_uint32, C.c_uint32, C.c_int, vp]),
     "qfm_dev_malloc": (vp, [C.c_size_t]),
     "qfm_dev_free": (C.c_int, [vp]),

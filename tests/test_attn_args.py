@@ -105,3 +105,39 @@ def test_attention_asks_for_its_workspace(lib):
     for args in ((0, 4, 8, 2, 10), (2, -1, 8, 2, 10), (2, 4, 7, 2, 10), (2, 4, 8, 65, 10), (2, 4, 8, 0, 10), (2, 4, 8, 2, -1)):
         assert lib.qfm_tree_attn_ws_bytes(C.byref(c), *args) == 0
     assert lib.qfm_tree_attn_ws_bytes(None, 2, 4, 8, 2, 10) == 0
+
+
+def _lora(**kw):
+    l = qfm.QfmLora()
+    l.n, l.K, l.R, l.slots, l.dtype, l.rank, l.scale = 2, 128, 16, 4, 1, P, P
+    for i in range(2):
+        l.a[i], l.b[i], l.base[i], l.y[i], l.rows[i] = P, P, P, P, 64
+    for k, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(l, k)[v[0]] = v[1]
+        else:
+            setattr(l, k, v)
+    return l
+
+
+def _lora_call(lib, l, x=P, xs=128, slot=P, T=4, ws=P, wsb=1 << 30):
+    return lib.qfm_lora_rows(C.byref(l) if l else None, x, xs, slot, T, ws, wsb, None), lib.qfm_last_error()
+
+
+def test_adapters_refuse(lib):
+    assert C.sizeof(qfm.QfmLora) == 184
+    for bad in (dict(n=0), dict(n=5), dict(K=0), dict(K=96), dict(K=1 << 17), dict(R=0), dict(R=12), dict(R=136), dict(slots=0),
+                dict(dtype=0), dict(dtype=3), dict(rank=None), dict(scale=None), dict(a=(1, None)), dict(b=(0, None)), dict(y=(1, None)),
+                dict(rows=(0, 0)), dict(rows=(1, -5)), dict(rows=(0, (1 << 20) + 1)), dict(a=(0, P + 8)), dict(y=(0, P + 4)),
+                dict(base=(1, P + 4))):
+        rc, msg = _lora_call(lib, _lora(**bad))
+        assert rc == -1 and b"qfm_lora_rows" in msg, bad
+    for bad in (dict(x=None), dict(x=P + 2), dict(xs=-8), dict(xs=132), dict(slot=None), dict(T=-1), dict(T=(1 << 20) + 1),
+                dict(ws=None), dict(wsb=4 * 2 * 16 * 4 - 1), dict(ws=P + 4)):
+        rc, msg = _lora_call(lib, _lora(), **bad)
+        assert rc == -1 and b"qfm_lora_rows" in msg, bad
+    assert _lora_call(lib, None)[0] == -1
+    assert _lora_call(lib, _lora(), T=0)[0] == 0
+    l = _lora()
+    assert lib.qfm_lora_ws_bytes(C.byref(l), 4) == 4 * 2 * 16 * 4 and lib.qfm_lora_ws_bytes(None, 4) == 0
+    assert lib.qfm_lora_ws_bytes(C.byref(_lora(R=12)), 4) == 0
