@@ -28,6 +28,8 @@
 namespace qfm {
 
 constexpr int kAttnWaves = 4;
+constexpr int kMaxSplits = 128;    // two a lane in the join
+constexpr long kMaxTokens = (1l << 31) - (1 << 16);   // 32 x a tile's number stays an int, past the last one too
 constexpr float kNoMax = -3.402823466e38f;
 constexpr float kLazy = 8.0f;      // the maximum may be exceeded by 2^8 before sums and results are rescaled
 constexpr int kVeMin = -118;       // least exponent of the value scale that the products are kept relative to
@@ -84,6 +86,13 @@ __device__ __forceinline__ void store4(uint8_t *out, long at, int dtype, float4 
     else *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_F16>(v.x, v.y), pack2<QFM_DT_F16>(v.z, v.w));
 }
 
+// a 32-token tile of keys and values, as the lanes hold it
+template <int NC>
+struct Tile {
+    u32x4_t k[2][NC], v[2][NC];
+    float4 ks[2], vs[2];
+};
+
 template <int FMT, int D, int RB, bool F32>
 __global__ void __launch_bounds__(64 * kAttnWaves)
 k_tree_attn(KvView c, AttnArgs a) {
@@ -91,15 +100,54 @@ k_tree_attn(KvView c, AttnArgs a) {
     __shared__ float s_o[kAttnWaves][ROWS * LD];
     __shared__ float s_m[kAttnWaves][ROWS], s_l[kAttnWaves][ROWS];
     __shared__ int s_ve[kAttnWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int g = lane >> 4, l16 = lane & 15;
     const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
     const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
     const int rows = sr.y * a.G, row0 = blk * ROWS;
     if (row0 >= rows) return;
-    const long cap = (long)c.max_pages << c.page_log2;
+    const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
     const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
     const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
     const int t1 = min(nt, ((int)blockIdx.x + 1) * per);
+    int t = (int)blockIdx.x * per + wave;
+
+    // the pages of a tile's halves (-1: none), requested a tile ahead; loads from page 0 in place of none
+    const int *table = c.table + (size_t)seq * c.max_pages;
+    auto pages = [&](int tt) {
+        const int p = 32 * tt, last = c.max_pages - 1;
+        int x = table[min(p >> c.page_log2, last)], y = table[min((p + 16) >> c.page_log2, last)];
+        x = p < len && (unsigned)x < (unsigned)c.n_pages ? x : -1;
+        y = p + 16 < len && (unsigned)y < (unsigned)c.n_pages ? y : -1;
+        return make_int2(x, y);
+    };
+    Tile<NC> w;
+    auto load_k = [&](int tt, int2 pg) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t at = c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                w.k[i][k] = *reinterpret_cast<const u32x4_t *>(c.k + at * D + l16 * D + 64 * k + 16 * g);
+            w.ks[i] = *reinterpret_cast<const float4 *>(c.ks + at + 4 * g);
+        }
+    };
+    auto load_v = [&](int tt, int2 pg) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t at = c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                w.v[i][k] = *reinterpret_cast<const u32x4_t *>(c.v + at * D + 4 * g * D + (64 * k + 4 * l16) * 4);
+            w.vs[i] = *reinterpret_cast<const float4 *>(c.vs + at + 4 * g);
+        }
+    };
+    int2 pg = pages(t);
+    if (t < t1) {
+        load_k(t, pg);
+        load_v(t, pg);
+    }
+    int2 pn = pages(t + kAttnWaves);
 
     // Q: fp16 fragments scaled per row, and what undoes the scaling
     f16x8_t qf[RB][NC][2][NP];
@@ -148,30 +196,14 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) o[rb][k][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int q = 0; q < 4; q++) o[rb][k][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    for (int t = (int)blockIdx.x * per + wave; t < t1; t += kAttnWaves) {
-        int page[2];
-        u32x4_t kr[2][NC], vr[2][NC];
-        float ks[2][4], vs[2][4];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int p = 32 * t + 16 * i;
-            page[i] = p < len ? c.page_of(seq, p) : -1;
-            const size_t at = c.token0(max(page[i], 0), h) + (p & (c.page() - 1));
-#pragma unroll
-            for (int k = 0; k < NC; k++)
-                kr[i][k] = *reinterpret_cast<const u32x4_t *>(c.k + (at + l16) * D + 64 * k + 16 * g);
-#pragma unroll
-            for (int k = 0; k < NC; k++)
-                vr[i][k] = *reinterpret_cast<const u32x4_t *>(c.v + (at + 4 * g) * D + (64 * k + 4 * l16) * 4);
-            const float4 x = *reinterpret_cast<const float4 *>(c.ks + at + 4 * g);
-            const float4 y = *reinterpret_cast<const float4 *>(c.vs + at + 4 * g);
-            ks[i][0] = x.x; ks[i][1] = x.y; ks[i][2] = x.z; ks[i][3] = x.w;
-            vs[i][0] = y.x; vs[i][1] = y.y; vs[i][2] = y.z; vs[i][3] = y.w;
-        }
-        // scores
+    // A tile's keys are used up before its values: the next keys are requested
+    // ahead of the softmax, the next values behind the second product, into the
+    // registers that have just become free.
+    while (t < t1) {
+        const bool more = t + kAttnWaves < t1;
         f32x4_t s[RB][2];
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) s[rb][0] = s[rb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -180,7 +212,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < NC; k++) {
                 f16x8_t ka, kb;
-                codes16<FMT>(kr[i][k], ka, kb);
+                codes16<FMT>(w.k[i][k], ka, kb);
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
@@ -190,16 +222,20 @@ k_tree_attn(KvView c, AttnArgs a) {
                     }
             }
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++)
+        for (int i = 0; i < 2; i++) {
+            const float ks[4] = {w.ks[i].x, w.ks[i].y, w.ks[i].z, w.ks[i].w};
 #pragma unroll
-            for (int i = 0; i < 2; i++)
+            for (int rb = 0; rb < RB; rb++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[i][e] * qs[rb];
-        const bool edge = 32 * t + 32 > ctx || page[0] < 0 || page[1] < 0;
+                for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[e];
+        }
+        if (more) load_k(t + kAttnWaves, pn);
+        float vs[2][4] = {{w.vs[0].x, w.vs[0].y, w.vs[0].z, w.vs[0].w}, {w.vs[1].x, w.vs[1].y, w.vs[1].z, w.vs[1].w}};
+        const bool edge = 32 * t + 32 > ctx || (pg.x | pg.y) < 0;
         if (edge) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const int j0 = 32 * t + 16 * i + 4 * g, n = page[i] < 0 ? 0 : min(max(len - j0, 0), 4);
+                const int j0 = 32 * t + 16 * i + 4 * g, n = (i ? pg.y : pg.x) < 0 ? 0 : min(max(len - j0, 0), 4);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     if (e >= n) vs[i][e] = 0.0f;
@@ -214,11 +250,11 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                     for (int k = 0; k < NC; k++)
 #pragma unroll
-                        for (int q = 0; q < 4; q++) vr[i][k][q] &= keep;
+                        for (int q = 0; q < 4; q++) w.v[i][k][q] &= keep;
                 }
             }
         }
-        // the largest score so far, and the largest value scale
+        // the largest score so far (base 2: times qs), and the largest value scale
         bool grow = false;
         float top[RB], vm = 0.0f;
 #pragma unroll
@@ -228,6 +264,7 @@ k_tree_attn(KvView c, AttnArgs a) {
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) top[rb] = fmaxf(top[rb], s[rb][i][e]);
+            top[rb] *= qs[rb];
             grow |= top[rb] > m[rb] + kLazy;
         }
 #pragma unroll
@@ -241,7 +278,7 @@ k_tree_attn(KvView c, AttnArgs a) {
             ve = vn;
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) {
-                const float mn = fmaxf(m[rb], max_over_g(top[rb])), f = exp2f(m[rb] - mn);
+                const float mn = fmaxf(m[rb], max_over_g(top[rb])), f = __builtin_amdgcn_exp2f(m[rb] - mn);
                 m[rb] = mn;
                 l[rb] *= f;
 #pragma unroll
@@ -262,7 +299,7 @@ k_tree_attn(KvView c, AttnArgs a) {
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float p = exp2f(s[rb][i][e] - m[rb]);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][i][e], qs[rb], -m[rb]));
                     l[rb] += p;
                     float x = p * vs[i][e];
                     if (edge && s[rb][i][e] == -INFINITY) x = 0.0f;   // not seen: its scale may be NaN
@@ -274,8 +311,8 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; k++) {
             f16x8_t a0, b0, a1, b1;
-            codes16<FMT>(vr[0][k], a0, b0);
-            codes16<FMT>(vr[1][k], a1, b1);
+            codes16<FMT>(w.v[0][k], a0, b0);
+            codes16<FMT>(w.v[1][k], a1, b1);
             const f16x8_t vf[4] = {__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 8, 9, 10, 11),
                                    __builtin_shufflevector(a0, a1, 4, 5, 6, 7, 12, 13, 14, 15),
                                    __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 8, 9, 10, 11),
@@ -287,6 +324,10 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                     for (int n = 0; n < NP; n++) o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], o[rb][k][q]);
         }
+        t += kAttnWaves;
+        if (more) load_v(t, pn);
+        pg = pn;
+        pn = pages(t + kAttnWaves);
     }
 
     // join the waves
@@ -348,42 +389,80 @@ k_tree_attn(KvView c, AttnArgs a) {
     }
 }
 
-// out(t, h) = sum_s w_s o_s / sum_s w_s, w_s = sum_s 2^(max_s - max): 256 / (D / 4)
-// heads a block.
+// out(t, h) = sum_s w_s o_s / sum_s w_s, w_s = sum_s 2^(max_s - max): one block a
+// row and head, a thread 4 channels of every (1024 / D)-th split.
 template <int D>
 __global__ void __launch_bounds__(256)
 k_tree_join(AttnArgs a, int heads) {
+    constexpr int TD = D / 4, NG = 256 / TD;
+    __shared__ float s_w[kMaxSplits], s_part[NG][D];
     const int2 sr = seq_rows(a.row_start, (int)blockIdx.z, a.T, a.max_nodes);
-    const int head = (int)blockIdx.x * (1024 / D) + (int)threadIdx.x / (D / 4), d = (int)threadIdx.x % (D / 4) * 4;
-    if ((int)blockIdx.y >= sr.y || head >= heads) return;
+    if ((int)blockIdx.y >= sr.y) return;
+    const int head = (int)blockIdx.x, d = (int)threadIdx.x % TD * 4, grp = (int)threadIdx.x / TD, lane = threadIdx.x & 63;
     const long t = sr.x + (int)blockIdx.y;
-    float mn = kNoMax, sum = 0.0f;
-    for (int s = 0; s < a.splits; s++) mn = fmaxf(mn, a.pml[((size_t)s * a.T + t) * heads + head].x);
+    const size_t row = (size_t)t * heads + head, step = (size_t)a.T * heads;
+    // every wave finds the weights, two splits a lane
+    float2 ml[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) ml[i] = lane + 64 * i < a.splits ? a.pml[(lane + 64 * i) * step + row] : make_float2(kNoMax, 0.0f);
+    constexpr int U = 8;
+    float4 y[U];
+#pragma unroll
+    for (int i = 0; i < U; i++)
+        if (grp + NG * i < a.splits) y[i] = *reinterpret_cast<const float4 *>(a.po + ((grp + NG * i) * step + row) * D + d);
+    float mn = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o));
+    const float w0 = ml[0].y * __builtin_amdgcn_exp2f(ml[0].x - mn), w1 = ml[1].y * __builtin_amdgcn_exp2f(ml[1].x - mn);
+    float sum = w0 + w1;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (threadIdx.x < 64) {
+        s_w[lane] = w0;
+        s_w[lane + 64] = w1;
+    }
+    __syncthreads();
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; s++) {
-        const size_t at = ((size_t)s * a.T + t) * heads + head;
-        const float2 ml = a.pml[at];
-        const float4 y = *reinterpret_cast<const float4 *>(a.po + at * D + d);
-        const float w = ml.y * exp2f(ml.x - mn);
-        if (ml.y == 0.0f) continue;
-        sum += w;
-        x.x = fmaf(w, y.x, x.x); x.y = fmaf(w, y.y, x.y); x.z = fmaf(w, y.z, x.z); x.w = fmaf(w, y.w, x.w);
+    for (int s0 = 0; s0 < a.splits; s0 += U * NG) {
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int s = s0 + grp + NG * i;
+            const float w = s < a.splits ? s_w[s] : 0.0f;
+            if (w == 0.0f) continue;                        // a split without keys wrote no result
+            x.x = fmaf(w, y[i].x, x.x); x.y = fmaf(w, y[i].y, x.y); x.z = fmaf(w, y[i].z, x.z); x.w = fmaf(w, y[i].w, x.w);
+        }
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int s = s0 + U * NG + grp + NG * i;
+            if (s < a.splits) y[i] = *reinterpret_cast<const float4 *>(a.po + (s * step + row) * D + d);
+        }
+    }
+    *reinterpret_cast<float4 *>(&s_part[grp][d]) = x;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int i = 1; i < NG; i++) {
+        const float4 z = *reinterpret_cast<const float4 *>(&s_part[i][d]);
+        x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-// 16-row blocks a workgroup takes: as many as the rows fill, within the
-// registers (64 results a lane and 64 channels of 16 rows)
-static int row_blocks(int D, int rows) { return rows <= 16 ? 1 : rows <= 32 || D == 256 ? 2 : 4; }
+// 16-row blocks a workgroup takes: as many as the rows fill and the registers
+// hold (F32 rows: twice the fragments of Q)
+constexpr int row_blocks(int D, int rows, bool f32) {
+    const int most = D == 64 ? 4 : D == 128 ? (f32 ? 2 : 4) : f32 ? 1 : 2, want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+    return want < most ? want : most;
+}
 
 // workgroups that share a sequence's keys: enough for the GPU's 256 CUs, each
 // with a tile or more for every wave
-static int attn_splits(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx) {
-    const int rows = max_nodes * (q_heads / kv_heads), per = 16 * row_blocks(D, rows);
+static int attn_splits(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, bool f32) {
+    const int rows = max_nodes * (q_heads / kv_heads), per = 16 * row_blocks(D, rows, f32);
     const long groups = (long)n_seq * kv_heads * ((rows + per - 1) / per);
     const long tiles = ((long)max_ctx + max_nodes + 31) / 32;
-    return (int)max(1l, min((long)min(128l, (768 + groups - 1) / groups), (tiles + kAttnWaves - 1) / kAttnWaves));
+    return (int)max(1l, min(min((long)kMaxSplits, (768 + groups - 1) / groups), (tiles + kAttnWaves - 1) / kAttnWaves));
 }
 
 static int attn_shape(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
@@ -398,16 +477,20 @@ static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
     return splits == 1 ? 0 : (size_t)splits * T * q_heads * (c->head_dim + 2) * 4;
 }
 
-template <int FMT, int D, int RB>
-static void attn_launch(const KvView &v, const AttnArgs &a, dim3 g, hipStream_t s) {
-    if (a.dtype == QFM_DT_F32) hipLaunchKernelGGL((k_tree_attn<FMT, D, RB, true>), g, dim3(64 * kAttnWaves), 0, s, v, a);
-    else hipLaunchKernelGGL((k_tree_attn<FMT, D, RB, false>), g, dim3(64 * kAttnWaves), 0, s, v, a);
+template <int FMT, int D, bool F32>
+static void attn_launch(const KvView &v, const AttnArgs &a, int rb, dim3 g, hipStream_t s) {
+    constexpr int MOST = row_blocks(D, 64, F32);
+    const dim3 b(64 * kAttnWaves);
+    if (rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, F32>), g, b, 0, s, v, a);
+    else if constexpr (MOST >= 2) {
+        if (rb == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, F32>), g, b, 0, s, v, a);
+        else if constexpr (MOST >= 4) hipLaunchKernelGGL((k_tree_attn<FMT, D, 4, F32>), g, b, 0, s, v, a);
+    }
 }
 template <int FMT, int D>
 static void attn_launch(const KvView &v, const AttnArgs &a, int rb, dim3 g, hipStream_t s) {
-    if (rb == 1) attn_launch<FMT, D, 1>(v, a, g, s);
-    else if (rb == 2) attn_launch<FMT, D, 2>(v, a, g, s);
-    else if constexpr (D != 256) attn_launch<FMT, D, 4>(v, a, g, s);
+    if (a.dtype == QFM_DT_F32) attn_launch<FMT, D, true>(v, a, rb, g, s);
+    else attn_launch<FMT, D, false>(v, a, rb, g, s);
 }
 
 }  // namespace qfm
@@ -418,7 +501,8 @@ extern "C" {
 
 size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
     if (attn_shape(c, n_seq, T, q_heads, max_nodes, max_ctx)) return 0;
-    return attn_ws(c, attn_splits(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx), T, q_heads);
+    // of the types' row blocks the larger ones make the fewer groups, and so the more splits
+    return attn_ws(c, attn_splits(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, false), T, q_heads);
 }
 
 int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, void *out, int dtype, int q_heads,
@@ -449,8 +533,8 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
         return -1;
     }
     if (!(scale > 0.0f) || !(scale < 3.4e38f)) { set_error(-1, "%s: scale %g", who, (double)scale); return -1; }
-    const int D = c->head_dim, G = q_heads / c->kv_heads, rb = row_blocks(D, max_nodes * G);
-    const int splits = attn_splits(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx);
+    const int D = c->head_dim, G = q_heads / c->kv_heads, rb = row_blocks(D, max_nodes * G, dtype == QFM_DT_F32);
+    const int splits = attn_splits(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype == QFM_DT_F32);
     const size_t need = attn_ws(c, splits, T, q_heads);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) & 15)) {
         set_error(-1, "%s: workspace of %zu bytes (16-byte aligned), %zu needed", who, ws ? ws_bytes : (size_t)0, need);
@@ -470,7 +554,7 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
     }
     if (check_launch(who)) return -3;
     if (splits > 1) {
-        const dim3 gj((unsigned)((q_heads + 1024 / D - 1) / (1024 / D)), (unsigned)max_nodes, (unsigned)sq->n_seq);
+        const dim3 gj((unsigned)q_heads, (unsigned)max_nodes, (unsigned)sq->n_seq);
         if (D == 64) hipLaunchKernelGGL(k_tree_join<64>, gj, dim3(256), 0, s, a, q_heads);
         else if (D == 128) hipLaunchKernelGGL(k_tree_join<128>, gj, dim3(256), 0, s, a, q_heads);
         else hipLaunchKernelGGL(k_tree_join<256>, gj, dim3(256), 0, s, a, q_heads);
