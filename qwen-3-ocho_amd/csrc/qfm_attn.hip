@@ -149,14 +149,18 @@ k_tree_attn(KvView c, AttnArgs a) {
     }
     int2 pn = pages(t + kAttnWaves);
 
-    // Q: fp16 fragments scaled per row, and what undoes the scaling
-    f16x8_t qf[RB][NC][2][NP];
-    float qs[RB];
+    // Q: fp16 fragments scaled per row, and what undoes the scaling; the waves
+    // share the row blocks out and leave them in LDS, in lane order
+    f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][NP][64]
+    auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * NP + n) << 6) + lane; };
     uint64_t see[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
-        const int r = row0 + 16 * rb + l16, rr = min(r, rows - 1), node = rr / a.G;
-        const uint8_t *p = a.q + ((sr.x + node) * a.qrs + (long)(h * a.G + rr - node * a.G) * a.qhs) * (F32 ? 4 : 2);
+        const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
+        see[rb] = a.tree ? a.tree[sr.x + node] : node == 63 ? ~0ull : (2ull << node) - 1;
+        if (RB > 1 && (rb & (kAttnWaves - 1)) != wave) continue;
+        if (RB == 1 && wave != 0) continue;
+        const uint8_t *p = a.q + ((sr.x + node) * a.qrs + (long)(h * a.G + r - node * a.G) * a.qhs) * (F32 ? 4 : 2);
         float v[NC][2][8], m = 0.0f;
 #pragma unroll
         for (int k = 0; k < NC; k++)
@@ -171,20 +175,43 @@ k_tree_attn(KvView c, AttnArgs a) {
             }
         const int k2 = f16_exp(max_over_g(m));
         const float sc = exp2i(k2);
-        qs[rb] = exp2i(-k2) * (a.scale * 1.4426950408889634f);
-        see[rb] = a.tree ? a.tree[sr.x + node] : node == 63 ? ~0ull : (2ull << node) - 1;
+        if (g == 0) s_m[0][16 * rb + l16] = exp2i(-k2) * (a.scale * 1.4426950408889634f);
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                f16x8_t hi, lo;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const float x = v[k][j][e] * sc;
-                    const _Float16 hi = (_Float16)x;
-                    qf[rb][k][j][0][e] = hi;
-                    if constexpr (F32) qf[rb][k][j][NP - 1][e] = (_Float16)(x - (float)hi);
+                    hi[e] = (_Float16)x;
+                    lo[e] = (_Float16)(x - (float)hi[e]);
                 }
+                s_q[frag(rb, k, j, 0)] = hi;
+                if constexpr (F32) s_q[frag(rb, k, j, NP - 1)] = lo;
+            }
     }
+    __syncthreads();
+    float qs[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) qs[rb] = s_m[0][16 * rb + l16];
+    // up to 32 registers of Q stay there, more are read from LDS tile by tile
+    constexpr bool QREG = RB * NC * 2 * NP * 4 <= 32;
+    f16x8_t qf[QREG ? RB : 1][QREG ? NC : 1][2][NP];
+    if constexpr (QREG) {
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int n = 0; n < NP; n++) qf[rb][k][j][n] = s_q[frag(rb, k, j, n)];
+    }
+    auto q_of = [&](int rb, int k, int j, int n, int at) {
+        if constexpr (QREG) return qf[rb][k][j][n];
+        else return s_q[frag(rb, k, j, n) + at];
+    };
 
     f32x4_t o[RB][NC][4];
     float m[RB], l[RB];
@@ -204,6 +231,8 @@ k_tree_attn(KvView c, AttnArgs a) {
     // registers that have just become free.
     while (t < t1) {
         const bool more = t + kAttnWaves < t1;
+        int again = 0;                     // what the compiler cannot see through: Q is not to be kept in registers
+        asm volatile("" : "+v"(again));
         f32x4_t s[RB][2];
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) s[rb][0] = s[rb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -214,12 +243,12 @@ k_tree_attn(KvView c, AttnArgs a) {
                 f16x8_t ka, kb;
                 codes16<FMT>(w.k[i][k], ka, kb);
 #pragma unroll
-                for (int rb = 0; rb < RB; rb++)
+                for (int n = 0; n < NP; n++) {
 #pragma unroll
-                    for (int n = 0; n < NP; n++) {
-                        s[rb][i] = mfma_f16(ka, qf[rb][k][0][n], s[rb][i]);
-                        s[rb][i] = mfma_f16(kb, qf[rb][k][1][n], s[rb][i]);
-                    }
+                    for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(ka, q_of(rb, k, 0, n, again), s[rb][i]);
+#pragma unroll
+                    for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(kb, q_of(rb, k, 1, n, again), s[rb][i]);
+                }
             }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -238,11 +267,17 @@ k_tree_attn(KvView c, AttnArgs a) {
                 const int j0 = 32 * t + 16 * i + 4 * g, n = (i ? pg.y : pg.x) < 0 ? 0 : min(max(len - j0, 0), 4);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    if (e >= n) vs[i][e] = 0.0f;
+                    // a value that is NaN reaches the rows that see it through their scores
+                    const bool lost = vs[i][e] != vs[i][e];
+                    const uint32_t nan = lost ? 0x7FC00000u : 0u;
+                    vs[i][e] = e >= n || lost ? 0.0f : vs[i][e];
+                    const int j = j0 + e - ctx;
+                    const uint64_t bit = 1ull << (j & 63);
 #pragma unroll
                     for (int rb = 0; rb < RB; rb++) {
-                        const int j = j0 + e - ctx;
-                        if (e >= n || (j >= 0 && !(see[rb] >> j & 1))) s[rb][i][e] = -INFINITY;
+                        const bool hide = (e >= n) | ((j >= 0) & ((see[rb] & bit) == 0));
+                        const float x = __uint_as_float(__float_as_uint(s[rb][i][e]) | nan);
+                        s[rb][i][e] = hide ? -INFINITY : x;
                     }
                 }
                 if constexpr (FMT == QFM_KV_E4M3) {       // a NaN code times 0 would be NaN
@@ -301,8 +336,7 @@ k_tree_attn(KvView c, AttnArgs a) {
                 for (int e = 0; e < 4; e++) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][i][e], qs[rb], -m[rb]));
                     l[rb] += p;
-                    float x = p * vs[i][e];
-                    if (edge && s[rb][i][e] == -INFINITY) x = 0.0f;   // not seen: its scale may be NaN
+                    const float x = p * vs[i][e];
                     const _Float16 hi = (_Float16)x;
                     pf[rb][0][4 * i + e] = hi;
                     if constexpr (F32) pf[rb][NP - 1][4 * i + e] = (_Float16)(x - (float)hi);
@@ -331,6 +365,7 @@ k_tree_attn(KvView c, AttnArgs a) {
     }
 
     // join the waves
+    __syncthreads();                       // Q has been read
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         l[rb] = sum_over_g(l[rb]);
