@@ -78,12 +78,154 @@ __device__ __forceinline__ float sum_over_g(float v) {
 }
 __device__ __forceinline__ float pow2_ratio(int d) { return d < -126 ? 0.0f : exp2i(min(d, 127)); }
 
+// the bytes of the first n of four tokens: a NaN code of E4M3 behind them would
+// make NaN of a product with 0
+__device__ __forceinline__ uint32_t token_bytes(int n) { return n == 4 ? ~0u : (1u << (8 * n)) - 1u; }
+
 // 4 values rounded to dtype
 __device__ __forceinline__ void store4(uint8_t *out, long at, int dtype, float4 v) {
     if (dtype == QFM_DT_F32) *reinterpret_cast<float4 *>(out + at * 4) = v;
     else if (dtype == QFM_DT_BF16)
         *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_BF16>(v.x, v.y), pack2<QFM_DT_BF16>(v.z, v.w));
     else *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_F16>(v.x, v.y), pack2<QFM_DT_F16>(v.z, v.w));
+}
+
+// One wave's rows: running maximum (base 2), sum and result, and the softmax
+// step of a tile. Result element i of o[rb][k][q] is channel 64 k + 16 g + 4 i + q
+// of row l16 of block rb.
+template <int RB, int NC, int NP>
+struct Rows {
+    f32x4_t o[RB][NC][4];
+    float m[RB], l[RB], qs[RB];
+    uint64_t see[RB];
+    int ve;
+    __device__ __forceinline__ void clear() {
+        ve = kVeMin;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            m[rb] = kNoMax;
+            l[rb] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) o[rb][k][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // scores s of tokens 4 g + e of half i, without the scales; n4[i]: how many of
+    // this lane's four tokens exist, j0[i]: the first one's node number
+    __device__ __forceinline__ void hide(f32x4_t (&s)[RB][2], float (&vs)[2][4], const int (&n4)[2], const int (&j0)[2]) const {
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                // a value that is NaN reaches the rows that see it through their scores
+                const bool lost = vs[i][e] != vs[i][e];
+                const uint32_t nan = lost ? 0x7FC00000u : 0u;
+                vs[i][e] = ((e >= n4[i]) | lost) ? 0.0f : vs[i][e];
+                const int j = j0[i] + e;
+                const uint64_t bit = 1ull << (j & 63);
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++) {
+                    const bool no = (e >= n4[i]) | ((j >= 0) & ((see[rb] & bit) == 0));
+                    const float x = __uint_as_float(__float_as_uint(s[rb][i][e]) | nan);
+                    s[rb][i][e] = no ? -INFINITY : x;
+                }
+            }
+    }
+    // p times the value scales, as the second product's operand
+    __device__ __forceinline__ void step(const f32x4_t (&s)[RB][2], float (&vs)[2][4], f16x8_t (&pf)[RB][NP]) {
+        bool grow = false;
+        float top[RB], vm = 0.0f;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            top[rb] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) top[rb] = fmaxf(top[rb], s[rb][i][e]);
+            top[rb] *= qs[rb];
+            grow |= top[rb] > m[rb] + kLazy;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vm = fmaxf(vm, vs[i][e]);
+        grow |= vm >= exp2i(ve) * 2.0f;
+        if (__any(grow)) {
+            const int vn = max(ve, (int)(__float_as_uint(max_over_g(vm)) >> 23) - 127);
+            const float vf = pow2_ratio(ve - vn);
+            ve = vn;
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) {
+                const float mn = fmaxf(m[rb], max_over_g(top[rb])), f = __builtin_amdgcn_exp2f(m[rb] - mn);
+                m[rb] = mn;
+                l[rb] *= f;
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) o[rb][k][q] *= f * vf;
+            }
+        }
+        const float vi = exp2i(6 - ve);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) vs[i][e] *= vi;
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][i][e], qs[rb], -m[rb]));
+                    l[rb] += p;
+                    const float x = p * vs[i][e];
+                    const _Float16 hi = (_Float16)x;
+                    pf[rb][0][4 * i + e] = hi;
+                    if constexpr (NP == 2) pf[rb][1][4 * i + e] = (_Float16)(x - (float)hi);
+                }
+    }
+};
+
+// a row's 16 NC values of this lane (channels 64 k + 16 g + 8 j + e) as fp16
+// fragments scaled by a power of two; returns what undoes it, times scale log2(e)
+template <int NC, int NP>
+__device__ __forceinline__ float q_frags(const AttnArgs &a, const uint8_t *p, int g, f16x8_t (&f)[NC][2][NP]) {
+    constexpr bool F32 = NP == 2;
+    float v[NC][2][8], m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NC; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint8_t *at = p + (64 * k + 16 * g + 8 * j) * (F32 ? 4 : 2);
+            if constexpr (F32) load8<QFM_DT_F32>(at, v[k][j]);
+            else if (a.dtype == QFM_DT_BF16) load8<QFM_DT_BF16>(at, v[k][j]);
+            else load8<QFM_DT_F16>(at, v[k][j]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
+        }
+    const int k2 = f16_exp(max_over_g(m));
+    const float sc = exp2i(k2);
+#pragma unroll
+    for (int k = 0; k < NC; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = v[k][j][e] * sc;
+                f[k][j][0][e] = (_Float16)x;
+                if constexpr (F32) f[k][j][1][e] = (_Float16)(x - (float)(_Float16)x);
+            }
+    return exp2i(-k2) * (a.scale * 1.4426950408889634f);
+}
+
+// where row r (node r / G, head r % G of the group) of a sequence lies in q
+template <bool F32>
+__device__ __forceinline__ const uint8_t *q_row(const AttnArgs &a, int first, int h, int r, int node) {
+    return a.q + ((first + node) * a.qrs + (long)(h * a.G + r - node * a.G) * a.qhs) * (F32 ? 4 : 2);
+}
+__device__ __forceinline__ uint64_t node_mask(const AttnArgs &a, int first, int node) {
+    return a.tree ? a.tree[first + node] : node == 63 ? ~0ull : (2ull << node) - 1;
 }
 
 // a 32-token tile of keys and values, as the lanes hold it
@@ -153,48 +295,25 @@ k_tree_attn(KvView c, AttnArgs a) {
     // share the row blocks out and leave them in LDS, in lane order
     f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][NP][64]
     auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * NP + n) << 6) + lane; };
-    uint64_t see[RB];
+    Rows<RB, NC, NP> R;
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
-        see[rb] = a.tree ? a.tree[sr.x + node] : node == 63 ? ~0ull : (2ull << node) - 1;
-        if (RB > 1 && (rb & (kAttnWaves - 1)) != wave) continue;
-        if (RB == 1 && wave != 0) continue;
-        const uint8_t *p = a.q + ((sr.x + node) * a.qrs + (long)(h * a.G + r - node * a.G) * a.qhs) * (F32 ? 4 : 2);
-        float v[NC][2][8], m = 0.0f;
+        R.see[rb] = node_mask(a, sr.x, node);
+        if ((rb & (kAttnWaves - 1)) != wave) continue;
+        f16x8_t f[NC][2][NP];
+        const float undo = q_frags<NC, NP>(a, q_row<F32>(a, sr.x, h, r, node), g, f);
+        if (g == 0) s_m[0][16 * rb + l16] = undo;
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const uint8_t *at = p + (64 * k + 16 * g + 8 * j) * (F32 ? 4 : 2);
-                if constexpr (F32) load8<QFM_DT_F32>(at, v[k][j]);
-                else if (a.dtype == QFM_DT_BF16) load8<QFM_DT_BF16>(at, v[k][j]);
-                else load8<QFM_DT_F16>(at, v[k][j]);
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
-            }
-        const int k2 = f16_exp(max_over_g(m));
-        const float sc = exp2i(k2);
-        if (g == 0) s_m[0][16 * rb + l16] = exp2i(-k2) * (a.scale * 1.4426950408889634f);
-#pragma unroll
-        for (int k = 0; k < NC; k++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                f16x8_t hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const float x = v[k][j][e] * sc;
-                    hi[e] = (_Float16)x;
-                    lo[e] = (_Float16)(x - (float)hi[e]);
-                }
-                s_q[frag(rb, k, j, 0)] = hi;
-                if constexpr (F32) s_q[frag(rb, k, j, NP - 1)] = lo;
-            }
+                for (int n = 0; n < NP; n++) s_q[frag(rb, k, j, n)] = f[k][j][n];
     }
     __syncthreads();
-    float qs[RB];
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) qs[rb] = s_m[0][16 * rb + l16];
+    for (int rb = 0; rb < RB; rb++) R.qs[rb] = s_m[0][16 * rb + l16];
     // up to 32 registers of Q stay there, more are read from LDS tile by tile
     constexpr bool QREG = RB * NC * 2 * NP * 4 <= 32;
     f16x8_t qf[QREG ? RB : 1][QREG ? NC : 1][2][NP];
@@ -213,19 +332,7 @@ k_tree_attn(KvView c, AttnArgs a) {
         else return s_q[frag(rb, k, j, n) + at];
     };
 
-    f32x4_t o[RB][NC][4];
-    float m[RB], l[RB];
-    int ve = kVeMin;
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-        m[rb] = kNoMax;
-        l[rb] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < NC; k++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) o[rb][k][q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    }
-
+    R.clear();
     // A tile's keys are used up before its values: the next keys are requested
     // ahead of the softmax, the next values behind the second product, into the
     // registers that have just become free.
@@ -260,87 +367,22 @@ k_tree_attn(KvView c, AttnArgs a) {
         }
         if (more) load_k(t + kAttnWaves, pn);
         float vs[2][4] = {{w.vs[0].x, w.vs[0].y, w.vs[0].z, w.vs[0].w}, {w.vs[1].x, w.vs[1].y, w.vs[1].z, w.vs[1].w}};
-        const bool edge = 32 * t + 32 > ctx || (pg.x | pg.y) < 0;
-        if (edge) {
+        if (32 * t + 32 > ctx || (pg.x | pg.y) < 0) {
+            const int j0[2] = {32 * t + 4 * g, 32 * t + 16 + 4 * g};
+            const int n4[2] = {pg.x < 0 ? 0 : min(max(len - j0[0], 0), 4), pg.y < 0 ? 0 : min(max(len - j0[1], 0), 4)};
+            const int node0[2] = {j0[0] - ctx, j0[1] - ctx};
+            R.hide(s, vs, n4, node0);
+            if constexpr (FMT == QFM_KV_E4M3) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int j0 = 32 * t + 16 * i + 4 * g, n = (i ? pg.y : pg.x) < 0 ? 0 : min(max(len - j0, 0), 4);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    // a value that is NaN reaches the rows that see it through their scores
-                    const bool lost = vs[i][e] != vs[i][e];
-                    const uint32_t nan = lost ? 0x7FC00000u : 0u;
-                    vs[i][e] = e >= n || lost ? 0.0f : vs[i][e];
-                    const int j = j0 + e - ctx;
-                    const uint64_t bit = 1ull << (j & 63);
-#pragma unroll
-                    for (int rb = 0; rb < RB; rb++) {
-                        const bool hide = (e >= n) | ((j >= 0) & ((see[rb] & bit) == 0));
-                        const float x = __uint_as_float(__float_as_uint(s[rb][i][e]) | nan);
-                        s[rb][i][e] = hide ? -INFINITY : x;
-                    }
-                }
-                if constexpr (FMT == QFM_KV_E4M3) {       // a NaN code times 0 would be NaN
-                    const uint32_t keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+                for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int k = 0; k < NC; k++)
 #pragma unroll
-                        for (int q = 0; q < 4; q++) w.v[i][k][q] &= keep;
-                }
+                        for (int q = 0; q < 4; q++) w.v[i][k][q] &= token_bytes(n4[i]);
             }
         }
-        // the largest score so far (base 2: times qs), and the largest value scale
-        bool grow = false;
-        float top[RB], vm = 0.0f;
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++) {
-            top[rb] = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) top[rb] = fmaxf(top[rb], s[rb][i][e]);
-            top[rb] *= qs[rb];
-            grow |= top[rb] > m[rb] + kLazy;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) vm = fmaxf(vm, vs[i][e]);
-        grow |= vm >= exp2i(ve) * 2.0f;
-        if (__any(grow)) {
-            const int vn = max(ve, (int)(__float_as_uint(max_over_g(vm)) >> 23) - 127);
-            const float vf = pow2_ratio(ve - vn);
-            ve = vn;
-#pragma unroll
-            for (int rb = 0; rb < RB; rb++) {
-                const float mn = fmaxf(m[rb], max_over_g(top[rb])), f = __builtin_amdgcn_exp2f(m[rb] - mn);
-                m[rb] = mn;
-                l[rb] *= f;
-#pragma unroll
-                for (int k = 0; k < NC; k++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++) o[rb][k][q] *= f * vf;
-            }
-        }
-        const float vi = exp2i(6 - ve);
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) vs[i][e] *= vi;
         f16x8_t pf[RB][NP];
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][i][e], qs[rb], -m[rb]));
-                    l[rb] += p;
-                    const float x = p * vs[i][e];
-                    const _Float16 hi = (_Float16)x;
-                    pf[rb][0][4 * i + e] = hi;
-                    if constexpr (F32) pf[rb][NP - 1][4 * i + e] = (_Float16)(x - (float)hi);
-                }
+        R.step(s, vs, pf);
         // results
 #pragma unroll
         for (int k = 0; k < NC; k++) {
@@ -356,7 +398,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
-                    for (int n = 0; n < NP; n++) o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], o[rb][k][q]);
+                    for (int n = 0; n < NP; n++) R.o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], R.o[rb][k][q]);
         }
         t += kAttnWaves;
         if (more) load_v(t, pn);
@@ -368,31 +410,30 @@ k_tree_attn(KvView c, AttnArgs a) {
     __syncthreads();                       // Q has been read
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
-        l[rb] = sum_over_g(l[rb]);
+        R.l[rb] = sum_over_g(R.l[rb]);
         if (g == 0) {
-            s_m[wave][16 * rb + l16] = m[rb];
-            s_l[wave][16 * rb + l16] = l[rb];
+            s_m[wave][16 * rb + l16] = R.m[rb];
+            s_l[wave][16 * rb + l16] = R.l[rb];
         }
     }
-    if (lane == 0) s_ve[wave] = ve;
+    if (lane == 0) s_ve[wave] = R.ve;
     __syncthreads();
     int vn = s_ve[0];
 #pragma unroll
     for (int w = 1; w < kAttnWaves; w++) vn = max(vn, s_ve[w]);
-    const float vf = pow2_ratio(ve - vn);
+    const float vf = pow2_ratio(R.ve - vn);
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         float mn = s_m[0][16 * rb + l16];
 #pragma unroll
         for (int w = 1; w < kAttnWaves; w++) mn = fmaxf(mn, s_m[w][16 * rb + l16]);
-        const float f = exp2f(m[rb] - mn) * vf;
-        // channel 64 k + 16 g + 4 i + q of row l16: element i of o[rb][k][q]
+        const float f = __builtin_amdgcn_exp2f(R.m[rb] - mn) * vf;
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
                 *reinterpret_cast<float4 *>(&s_o[wave][(16 * rb + l16) * LD + 64 * k + 16 * g + 4 * i]) =
-                    make_float4(o[rb][k][0][i] * f, o[rb][k][1][i] * f, o[rb][k][2][i] * f, o[rb][k][3][i] * f);
+                    make_float4(R.o[rb][k][0][i] * f, R.o[rb][k][1][i] * f, R.o[rb][k][2][i] * f, R.o[rb][k][3][i] * f);
     }
     __syncthreads();
     const float back = exp2i(vn - 6);
@@ -420,6 +461,273 @@ k_tree_attn(KvView c, AttnArgs a) {
             const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
             *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
             if (d == 0) a.pml[at] = make_float2(mn, sum);
+        }
+    }
+}
+
+// The same for many rows (more than kFewRows of a key/value head): eight waves,
+// 8 / WT of them with 16 RB rows each, in WT groups that take the tiles in turn.
+// A tile is widened to fp16 once, by all waves, and laid into LDS in the order
+// of the MFMA operands (16-byte reads and writes, no two lanes on a bank); each
+// step's tiles are requested a step ahead of being widened and widened a step
+// ahead of their use, one barrier a step.
+constexpr int kWideWaves = 8;
+
+template <int FMT, int D, int RB, bool F32, int WT>
+__global__ void __launch_bounds__(64 * kWideWaves)
+k_tree_wide(KvView c, AttnArgs a) {
+    constexpr int NC = D / 64, NP = F32 ? 2 : 1, WR = kWideWaves / WT, ROWS = 16 * RB * WR;
+    constexpr int NF = 8 * NC;                              // fragments a tile: 4 NC of K, then 4 NC of V
+    constexpr int UNITS = WT * 4 * NC, UN = (UNITS + kWideWaves - 1) / kWideWaves, LJ = 68;
+    constexpr int TILES = 2 * WT * NF * 64 * 16, JOIN = WT > 1 ? kWideWaves * 16 * RB * LJ * 4 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[TILES > JOIN ? TILES : JOIN];
+    __shared__ float s_sc[2][WT][64];                       // 32 key scales, 32 value scales
+    __shared__ float s_m[kWideWaves][16 * RB], s_l[kWideWaves][16 * RB];
+    __shared__ int s_ve[kWideWaves];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int g = lane >> 4, l16 = lane & 15, wr = wave % WR, wt = wave / WR;
+    const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
+    const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
+    const int rows = sr.y * a.G, row0 = blk * ROWS;
+    if (row0 >= rows) return;
+    const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
+    const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
+    const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
+    const int t0 = (int)blockIdx.x * per, t1 = min(nt, t0 + per), steps = (t1 - t0 + WT - 1) / WT;
+    const int lim = min(len, 32 * t1);                      // tokens from here on are no keys of this workgroup
+    const bool live = row0 + 16 * RB * wr < rows;           // this wave has rows
+
+    const int *table = c.table + (size_t)seq * c.max_pages;
+    auto pages = [&](int tt) {
+        const int p = 32 * tt, last = c.max_pages - 1;
+        int x = table[min(p >> c.page_log2, last)], y = table[min((p + 16) >> c.page_log2, last)];
+        x = p < lim && (unsigned)x < (unsigned)c.n_pages ? x : -1;
+        y = p + 16 < lim && (unsigned)y < (unsigned)c.n_pages ? y : -1;
+        return make_int2(x, y);
+    };
+    // token index of half i of tile tt, on page 0 where there is none
+    auto half_at = [&](int tt, int i, int2 pg) {
+        return c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
+    };
+    u32x4_t raw[UN];
+    float raw_sc;
+    auto request = [&](int step, const int2 (&pg)[WT]) {
+#pragma unroll
+        for (int n = 0; n < UN; n++) {
+            const int u = wave + kWideWaves * n, w = u / (4 * NC), r = u % (4 * NC), i = (r % (2 * NC)) / NC, k = r % NC;
+            if (u >= UNITS) break;
+            int2 p = pg[0];
+#pragma unroll
+            for (int v = 1; v < WT; v++) p = w == v ? pg[v] : p;
+            const size_t at = half_at(t0 + step * WT + w, i, p);
+            const uint8_t *src = r < 2 * NC ? c.k + at * D + l16 * D + 64 * k + 16 * g
+                                            : c.v + at * D + 4 * g * D + (64 * k + 4 * l16) * 4;
+            raw[n] = *reinterpret_cast<const u32x4_t *>(src);
+        }
+        if (wave < WT) {
+            int2 p = pg[0];
+#pragma unroll
+            for (int v = 1; v < WT; v++) p = wave == v ? pg[v] : p;
+            const int tt = t0 + step * WT + wave, i = (lane >> 4) & 1;
+            const size_t at = half_at(tt, i, p) + l16;
+            raw_sc = (lane < 32 ? c.ks : c.vs)[at];
+        }
+    };
+    auto widen = [&](int step, const int2 (&pg)[WT]) {
+        uint8_t *buf = s_buf + (step & 1) * (TILES / 2);
+#pragma unroll
+        for (int n = 0; n < UN; n++) {
+            const int u = wave + kWideWaves * n, w = u / (4 * NC), r = u % (4 * NC), i = (r % (2 * NC)) / NC, k = r % NC;
+            if (u >= UNITS) break;
+            uint8_t *dst = buf + (size_t)w * (NF * 1024) + lane * 16;
+            f16x8_t x, y;
+            if (r < 2 * NC) {
+                codes16<FMT>(raw[n], x, y);
+                *reinterpret_cast<f16x8_t *>(dst + ((i * NC + k) * 2) * 1024) = x;
+                *reinterpret_cast<f16x8_t *>(dst + ((i * NC + k) * 2 + 1) * 1024) = y;
+            } else {
+                if constexpr (FMT == QFM_KV_E4M3) {
+                    int2 p = pg[0];
+#pragma unroll
+                    for (int v = 1; v < WT; v++) p = w == v ? pg[v] : p;
+                    const int j0 = 32 * (t0 + step * WT + w) + 16 * i + 4 * g;
+                    const uint32_t keep = token_bytes((i ? p.y : p.x) < 0 ? 0 : min(max(lim - j0, 0), 4));
+#pragma unroll
+                    for (int q = 0; q < 4; q++) raw[n][q] &= keep;
+                }
+                codes16<FMT>(raw[n], x, y);
+                const u32x4_t p = __builtin_bit_cast(u32x4_t, x), q = __builtin_bit_cast(u32x4_t, y);
+                dst += (4 * NC + 4 * k) * 1024 + 8 * i;
+                *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{p[0], p[1]};
+                *reinterpret_cast<u32x2_t *>(dst + 1024) = u32x2_t{p[2], p[3]};
+                *reinterpret_cast<u32x2_t *>(dst + 2048) = u32x2_t{q[0], q[1]};
+                *reinterpret_cast<u32x2_t *>(dst + 3072) = u32x2_t{q[2], q[3]};
+            }
+        }
+        if (wave < WT) s_sc[step & 1][wave][lane] = raw_sc;
+    };
+    int2 pc[WT], pn[WT], pf2[WT];                           // pages of this step's tiles and of the next two
+#pragma unroll
+    for (int w = 0; w < WT; w++) {
+        pc[w] = pages(t0 + w);
+        pn[w] = pages(t0 + WT + w);
+        pf2[w] = pages(t0 + 2 * WT + w);
+    }
+    if (steps > 0) request(0, pc);
+
+    Rows<RB, NC, NP> R;
+    f16x8_t qf[RB][NC][2][NP];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        const int r = min(row0 + 16 * (RB * wr + rb) + l16, rows - 1), node = r / a.G;
+        R.see[rb] = node_mask(a, sr.x, node);
+        R.qs[rb] = q_frags<NC, NP>(a, q_row<F32>(a, sr.x, h, r, node), g, qf[rb]);
+    }
+    R.clear();
+    if (steps > 0) widen(0, pc);
+    if (steps > 1) request(1, pn);
+    __syncthreads();
+    for (int st = 0; st < steps; st++) {
+        if (st + 1 < steps) widen(st + 1, pn);
+        if (st + 2 < steps) request(st + 2, pf2);
+        if (live) {
+            const uint8_t *buf = s_buf + (st & 1) * (TILES / 2) + wt * (NF * 1024) + lane * 16;
+            const int t = t0 + st * WT + wt;
+            int2 pg = pc[0];
+#pragma unroll
+            for (int v = 1; v < WT; v++) pg = wt == v ? pc[v] : pg;
+            f32x4_t s[RB][2];
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++) s[rb][0] = s[rb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const f16x8_t kf = *reinterpret_cast<const f16x8_t *>(buf + ((i * NC + k) * 2 + j) * 1024);
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+#pragma unroll
+                            for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(kf, qf[rb][k][j][n], s[rb][i]);
+                    }
+            float vs[2][4];
+            const float *sc = s_sc[st & 1][wt];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float4 x = *reinterpret_cast<const float4 *>(sc + 16 * i + 4 * g);
+                const float4 y = *reinterpret_cast<const float4 *>(sc + 32 + 16 * i + 4 * g);
+                const float ks[4] = {x.x, x.y, x.z, x.w};
+                vs[i][0] = y.x; vs[i][1] = y.y; vs[i][2] = y.z; vs[i][3] = y.w;
+#pragma unroll
+                for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[e];
+            }
+            if (32 * t + 32 > min(ctx, lim) || (pg.x | pg.y) < 0) {
+                const int j0[2] = {32 * t + 4 * g, 32 * t + 16 + 4 * g};
+                const int n4[2] = {pg.x < 0 ? 0 : min(max(lim - j0[0], 0), 4), pg.y < 0 ? 0 : min(max(lim - j0[1], 0), 4)};
+                const int node0[2] = {j0[0] - ctx, j0[1] - ctx};
+                R.hide(s, vs, n4, node0);
+            }
+            f16x8_t pf[RB][NP];
+            R.step(s, vs, pf);
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f16x8_t vf = *reinterpret_cast<const f16x8_t *>(buf + (4 * NC + 4 * k + q) * 1024);
+#pragma unroll
+                    for (int n = 0; n < NP; n++)
+#pragma unroll
+                        for (int rb = 0; rb < RB; rb++) R.o[rb][k][q] = mfma_f16(vf, pf[rb][n], R.o[rb][k][q]);
+                }
+        }
+#pragma unroll
+        for (int w = 0; w < WT; w++) {
+            pc[w] = pn[w];
+            pn[w] = pf2[w];
+            pf2[w] = pages(t0 + (st + 3) * WT + w);
+        }
+        __syncthreads();
+    }
+
+    const int heads = c.heads * a.G;
+    auto put = [&](int r, int d, float4 x, float mn, float sum, bool first) {
+        const int node = r / a.G, head = h * a.G + r - node * a.G;
+        const long t = sr.x + node;
+        if (a.splits == 1) {
+            store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, x);
+        } else {
+            const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
+            *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
+            if (first) a.pml[at] = make_float2(mn, sum);
+        }
+    };
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) R.l[rb] = sum_over_g(R.l[rb]);
+    if constexpr (WT == 1) {
+        const float back = exp2i(R.ve - 6);
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            const int r = row0 + 16 * (RB * wr + rb) + l16;
+            const float inv = R.l[rb] == 0.0f ? 0.0f : back / R.l[rb];
+            if (r < rows)
+#pragma unroll
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        put(r, 64 * k + 16 * g + 4 * i, make_float4(R.o[rb][k][0][i] * inv, R.o[rb][k][1][i] * inv,
+                            R.o[rb][k][2][i] * inv, R.o[rb][k][3][i] * inv), R.m[rb], R.l[rb], k + g + i == 0);
+        }
+    } else {
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++)
+            if (g == 0) {
+                s_m[wave][16 * rb + l16] = R.m[rb];
+                s_l[wave][16 * rb + l16] = R.l[rb];
+            }
+        if (lane == 0) s_ve[wave] = R.ve;
+        __syncthreads();
+        int vn = s_ve[0];
+#pragma unroll
+        for (int w = 1; w < kWideWaves; w++) vn = max(vn, s_ve[w]);
+        float f[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; rb++) {
+            float mn = kNoMax;
+#pragma unroll
+            for (int w = 0; w < WT; w++) mn = fmaxf(mn, s_m[w * WR + wr][16 * rb + l16]);
+            f[rb] = __builtin_amdgcn_exp2f(R.m[rb] - mn) * pow2_ratio(R.ve - vn);
+        }
+        const float back = exp2i(vn - 6);
+        float *s_j = reinterpret_cast<float *>(s_buf);      // [waves][16 RB][LJ]: 64 channels at a time
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+#pragma unroll
+            for (int rb = 0; rb < RB; rb++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(&s_j[(wave * 16 * RB + 16 * rb + l16) * LJ + 16 * g + 4 * i]) =
+                        make_float4(R.o[rb][k][0][i] * f[rb], R.o[rb][k][1][i] * f[rb], R.o[rb][k][2][i] * f[rb], R.o[rb][k][3][i] * f[rb]);
+            __syncthreads();
+            for (int e = threadIdx.x; e < ROWS * 16; e += 64 * kWideWaves) {
+                const int r = e >> 4, d = (e & 15) * 4, rw = r / (16 * RB), rr = r % (16 * RB);
+                if (row0 + r >= rows) break;
+                float mn = kNoMax, sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WT; w++) mn = fmaxf(mn, s_m[w * WR + rw][rr]);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < WT; w++) {
+                    const float4 y = *reinterpret_cast<const float4 *>(&s_j[((w * WR + rw) * 16 * RB + rr) * LJ + d]);
+                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+                    sum += s_l[w * WR + rw][rr] * __builtin_amdgcn_exp2f(s_m[w * WR + rw][rr] - mn);
+                }
+                const float inv = sum == 0.0f ? 0.0f : back / sum;
+                put(row0 + r, 64 * k + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), mn, sum, k + d == 0);
+            }
+            __syncthreads();
         }
     }
 }
@@ -484,20 +792,39 @@ k_tree_join(AttnArgs a, int heads) {
     store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-// 16-row blocks a workgroup takes: as many as the rows fill and the registers
-// hold (F32 rows: twice the fragments of Q)
-constexpr int row_blocks(int D, int rows, bool f32) {
+// How a call is laid out: 16 RB rows a wave; few rows (wt 0) as k_tree_attn, more
+// as k_tree_wide with wt groups of waves; and the splits of a sequence's keys.
+struct AttnPlan { int rb, wt, block, splits; };      // block: rows a workgroup
+constexpr int kFewRows = 64;
+constexpr int few_blocks(int D, int rows, bool f32) {
     const int most = D == 64 ? 4 : D == 128 ? (f32 ? 2 : 4) : f32 ? 1 : 2, want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
     return want < most ? want : most;
 }
+// wide: the rows a wave holds within 256 registers
+constexpr int wide_blocks(int D, bool f32) { return D == 64 ? 2 : D == 128 && !f32 ? 2 : 1; }
+// workgroups that a CU holds at once
+constexpr int few_resident(int D, int rb) { return rb == 1 && D <= 128 ? 2 : rb == 2 && D == 64 ? 2 : 1; }
 
-// workgroups that share a sequence's keys: enough for the GPU's 256 CUs, each
-// with a tile or more for every wave
-static int attn_splits(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, bool f32) {
-    const int rows = max_nodes * (q_heads / kv_heads), per = 16 * row_blocks(D, rows, f32);
-    const long groups = (long)n_seq * kv_heads * ((rows + per - 1) / per);
-    const long tiles = ((long)max_ctx + max_nodes + 31) / 32;
-    return (int)max(1l, min(min((long)kMaxSplits, (768 + groups - 1) / groups), (tiles + kAttnWaves - 1) / kAttnWaves));
+static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, bool f32) {
+    const int rows = max_nodes * (q_heads / kv_heads);
+    AttnPlan p{};
+    int resident;
+    if (rows <= kFewRows) {
+        p.rb = few_blocks(D, rows, f32);
+        p.block = 16 * p.rb;
+        resident = few_resident(D, p.rb);
+    } else {
+        p.rb = wide_blocks(D, f32);
+        p.wt = rows <= 4 * 16 * p.rb ? 2 : 1;
+        p.block = 16 * p.rb * (kWideWaves / p.wt);
+        resident = 1;
+    }
+    // one round of resident workgroups over the 256 CUs, each with a tile or more
+    // for every wave (or group of waves)
+    const long groups = (long)n_seq * kv_heads * ((rows + p.block - 1) / p.block);
+    const long tiles = ((long)max_ctx + max_nodes + 31) / 32, each = p.wt ? 2 * p.wt : kAttnWaves;
+    p.splits = (int)max(1l, min(min((long)kMaxSplits, 256 * resident / groups), (tiles + each - 1) / each));
+    return p;
 }
 
 static int attn_shape(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
@@ -513,19 +840,26 @@ static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
 }
 
 template <int FMT, int D, bool F32>
-static void attn_launch(const KvView &v, const AttnArgs &a, int rb, dim3 g, hipStream_t s) {
-    constexpr int MOST = row_blocks(D, 64, F32);
+static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, dim3 g, hipStream_t s) {
+    if (p.wt) {
+        constexpr int RB = wide_blocks(D, F32);
+        const dim3 b(64 * kWideWaves);
+        if (p.wt == 1) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, F32, 1>), g, b, 0, s, v, a);
+        else hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, F32, 2>), g, b, 0, s, v, a);
+        return;
+    }
+    constexpr int MOST = few_blocks(D, kFewRows, F32);
     const dim3 b(64 * kAttnWaves);
-    if (rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, F32>), g, b, 0, s, v, a);
+    if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, F32>), g, b, 0, s, v, a);
     else if constexpr (MOST >= 2) {
-        if (rb == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, F32>), g, b, 0, s, v, a);
+        if (p.rb == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, F32>), g, b, 0, s, v, a);
         else if constexpr (MOST >= 4) hipLaunchKernelGGL((k_tree_attn<FMT, D, 4, F32>), g, b, 0, s, v, a);
     }
 }
 template <int FMT, int D>
-static void attn_launch(const KvView &v, const AttnArgs &a, int rb, dim3 g, hipStream_t s) {
-    if (a.dtype == QFM_DT_F32) attn_launch<FMT, D, true>(v, a, rb, g, s);
-    else attn_launch<FMT, D, false>(v, a, rb, g, s);
+static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, dim3 g, hipStream_t s) {
+    if (a.dtype == QFM_DT_F32) attn_launch<FMT, D, true>(v, a, p, g, s);
+    else attn_launch<FMT, D, false>(v, a, p, g, s);
 }
 
 }  // namespace qfm
@@ -536,8 +870,10 @@ extern "C" {
 
 size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
     if (attn_shape(c, n_seq, T, q_heads, max_nodes, max_ctx)) return 0;
-    // of the types' row blocks the larger ones make the fewer groups, and so the more splits
-    return attn_ws(c, attn_splits(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, false), T, q_heads);
+    int splits = 1;
+    for (int f32 = 0; f32 < 2; f32++)
+        splits = max(splits, attn_plan(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, f32).splits);
+    return attn_ws(c, splits, T, q_heads);
 }
 
 int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, void *out, int dtype, int q_heads,
@@ -568,8 +904,9 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
         return -1;
     }
     if (!(scale > 0.0f) || !(scale < 3.4e38f)) { set_error(-1, "%s: scale %g", who, (double)scale); return -1; }
-    const int D = c->head_dim, G = q_heads / c->kv_heads, rb = row_blocks(D, max_nodes * G, dtype == QFM_DT_F32);
-    const int splits = attn_splits(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype == QFM_DT_F32);
+    const int D = c->head_dim, G = q_heads / c->kv_heads;
+    const AttnPlan p = attn_plan(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype == QFM_DT_F32);
+    const int splits = p.splits;
     const size_t need = attn_ws(c, splits, T, q_heads);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) & 15)) {
         set_error(-1, "%s: workspace of %zu bytes (16-byte aligned), %zu needed", who, ws ? ws_bytes : (size_t)0, need);
@@ -580,12 +917,12 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
                q_row_stride, q_head_stride, out_row_stride, out_head_stride, row_start, ctx, tree, scale, nullptr, nullptr};
     a.po = static_cast<float *>(ws);
     if (splits > 1) a.pml = reinterpret_cast<float2 *>(a.po + (size_t)splits * T * q_heads * D);
-    const dim3 g((unsigned)splits, (unsigned)(c->kv_heads * ((max_nodes * G + 16 * rb - 1) / (16 * rb))), (unsigned)sq->n_seq);
+    const dim3 g((unsigned)splits, (unsigned)(c->kv_heads * ((max_nodes * G + p.block - 1) / p.block)), (unsigned)sq->n_seq);
     const bool i8 = c->fmt == QFM_KV_INT8;
     switch (D) {
-        case 64: i8 ? attn_launch<QFM_KV_INT8, 64>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 64>(v, a, rb, g, s); break;
-        case 128: i8 ? attn_launch<QFM_KV_INT8, 128>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 128>(v, a, rb, g, s); break;
-        default: i8 ? attn_launch<QFM_KV_INT8, 256>(v, a, rb, g, s) : attn_launch<QFM_KV_E4M3, 256>(v, a, rb, g, s); break;
+        case 64: i8 ? attn_launch<QFM_KV_INT8, 64>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 64>(v, a, p, g, s); break;
+        case 128: i8 ? attn_launch<QFM_KV_INT8, 128>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 128>(v, a, p, g, s); break;
+        default: i8 ? attn_launch<QFM_KV_INT8, 256>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 256>(v, a, p, g, s); break;
     }
     if (check_launch(who)) return -3;
     if (splits > 1) {

@@ -97,7 +97,12 @@ def _run(rng, c, counts, ctx, Hq, dt, tree=True, layout="rows", extra=0, scale=N
     ([2, 5], [40, 17], 8, 8, 64, 128, "heads"),             # every head its own
     ([64, 33], [95, 160], 8, 2, 128, 32, "rows"),           # the widest trees, several row blocks
     ([64], [7], 12, 4, 256, 256, "heads"),
-    ([64, 1, 20], [200, 3, 0], 16, 4, 64, 16, "rows")])
+    ([64, 1, 20], [200, 3, 0], 16, 4, 64, 16, "rows"),
+    ([20, 17], [700, 33], 16, 4, 128, 32, "wide"),          # 65 to 128 rows of a head
+    ([9, 1], [333, 1300], 16, 2, 256, 16, "rows"),
+    ([33, 30], [64, 900], 8, 2, 64, 64, "heads"),
+    ([41], [2100], 12, 4, 128, 16, "rows"),                 # more, keys split over workgroups
+    ([10, 16, 3], [50, 0, 40], 8, 2, 128, 32, "rows")])     # 33 to 64
 def test_against_64_bits(fmt, dt, counts, ctx, Hq, H, D, page, layout):
     _say("fmt", fmt, dt, "rows", counts, "ctx", ctx, "heads", Hq, H, "D", D, "page", page, layout)
     rng = np.random.default_rng(sum(ctx) + Hq * D + fmt)
