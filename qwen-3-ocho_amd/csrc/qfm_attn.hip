@@ -37,7 +37,7 @@ constexpr int kVeMin = -118;       // least exponent of the value scale that the
 struct AttnArgs {
     const uint8_t *q;
     uint8_t *out;
-    int dtype, G, T, max_nodes, splits;
+    int G, T, max_nodes, splits;
     long qrs, qhs, ors, ohs;
     const int *row_start, *ctx;
     const uint64_t *tree;
@@ -82,18 +82,21 @@ __device__ __forceinline__ float pow2_ratio(int d) { return d < -126 ? 0.0f : ex
 // make NaN of a product with 0
 __device__ __forceinline__ uint32_t token_bytes(int n) { return n == 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
-// 4 values rounded to dtype
-__device__ __forceinline__ void store4(uint8_t *out, long at, int dtype, float4 v) {
-    if (dtype == QFM_DT_F32) *reinterpret_cast<float4 *>(out + at * 4) = v;
-    else if (dtype == QFM_DT_BF16)
-        *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_BF16>(v.x, v.y), pack2<QFM_DT_BF16>(v.z, v.w));
-    else *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<QFM_DT_F16>(v.x, v.y), pack2<QFM_DT_F16>(v.z, v.w));
+// 4 values rounded to the type
+template <int DT>
+__device__ __forceinline__ void store4(uint8_t *out, long at, float4 v) {
+    if constexpr (DT == QFM_DT_F32) *reinterpret_cast<float4 *>(out + at * 4) = v;
+    else *reinterpret_cast<uint2 *>(out + at * 2) = make_uint2(pack2<DT>(v.x, v.y), pack2<DT>(v.z, v.w));
 }
 
 // One wave's rows: running maximum (base 2), sum and result, and the softmax
 // step of a tile. Result element i of o[rb][k][q] is channel 64 k + 16 g + 4 i + q
 // of row l16 of block rb.
-template <int RB, int NC, int NP>
+// how many fp16 numbers an element of Q and a weight p take
+constexpr int q_parts(int dt) { return dt == QFM_DT_F32 ? 2 : 1; }
+constexpr int p_parts(int dt) { return dt == QFM_DT_BF16 ? 1 : 2; }
+
+template <int RB, int NC, int PP>
 struct Rows {
     f32x4_t o[RB][NC][4];
     float m[RB], l[RB], qs[RB];
@@ -133,7 +136,7 @@ struct Rows {
             }
     }
     // p times the value scales, as the second product's operand
-    __device__ __forceinline__ void step(const f32x4_t (&s)[RB][2], float (&vs)[2][4], f16x8_t (&pf)[RB][NP]) {
+    __device__ __forceinline__ void step(const f32x4_t (&s)[RB][2], float (&vs)[2][4], f16x8_t (&pf)[RB][PP]) {
         bool grow = false;
         float top[RB], vm = 0.0f;
 #pragma unroll
@@ -182,48 +185,54 @@ struct Rows {
                     const float x = p * vs[i][e];
                     const _Float16 hi = (_Float16)x;
                     pf[rb][0][4 * i + e] = hi;
-                    if constexpr (NP == 2) pf[rb][1][4 * i + e] = (_Float16)(x - (float)hi);
+                    if constexpr (PP == 2) pf[rb][1][4 * i + e] = (_Float16)(x - (float)hi);
                 }
     }
 };
 
-// a row's 16 NC values of this lane (channels 64 k + 16 g + 8 j + e) as fp16
-// fragments scaled by a power of two; returns what undoes it, times scale log2(e)
-template <int NC, int NP>
-__device__ __forceinline__ float q_frags(const AttnArgs &a, const uint8_t *p, int g, f16x8_t (&f)[NC][2][NP]) {
-    constexpr bool F32 = NP == 2;
-    float v[NC][2][8], m = 0.0f;
+// A row's 16 NC values of this lane (channels 64 k + 16 g + 8 j + e): as they
+// come, then as fp16 fragments scaled by a power of two; widen() returns what
+// undoes it, times scale log2(e).
+template <int NC, int DT>
+struct QRow {
+    static constexpr int ES = DT == QFM_DT_F32 ? 4 : 2, QP = q_parts(DT);
+    u32x4_t raw[NC][2][ES / 2];
+    // row r (node r / G, head r % G of the group) of the sequence whose first row is `first`
+    __device__ __forceinline__ void load(const AttnArgs &a, int first, int h, int r, int node, int g) {
+        const uint8_t *p = a.q + ((first + node) * a.qrs + (long)(h * a.G + r - node * a.G) * a.qhs) * ES;
 #pragma unroll
-    for (int k = 0; k < NC; k++)
+        for (int k = 0; k < NC; k++)
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const uint8_t *at = p + (64 * k + 16 * g + 8 * j) * (F32 ? 4 : 2);
-            if constexpr (F32) load8<QFM_DT_F32>(at, v[k][j]);
-            else if (a.dtype == QFM_DT_BF16) load8<QFM_DT_BF16>(at, v[k][j]);
-            else load8<QFM_DT_F16>(at, v[k][j]);
+            for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
-        }
-    const int k2 = f16_exp(max_over_g(m));
-    const float sc = exp2i(k2);
+                for (int w = 0; w < ES / 2; w++)
+                    raw[k][j][w] = *reinterpret_cast<const u32x4_t *>(p + (64 * k + 16 * g + 8 * j) * ES + 16 * w);
+    }
+    __device__ __forceinline__ float widen(float scale, f16x8_t (&f)[NC][2][QP]) const {
+        float v[NC][2][8], m = 0.0f;
 #pragma unroll
-    for (int k = 0; k < NC; k++)
+        for (int k = 0; k < NC; k++)
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 2; j++) {
+                load8<DT>(&raw[k][j][0], v[k][j]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float x = v[k][j][e] * sc;
-                f[k][j][0][e] = (_Float16)x;
-                if constexpr (F32) f[k][j][1][e] = (_Float16)(x - (float)(_Float16)x);
+                for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
             }
-    return exp2i(-k2) * (a.scale * 1.4426950408889634f);
-}
-
-// where row r (node r / G, head r % G of the group) of a sequence lies in q
-template <bool F32>
-__device__ __forceinline__ const uint8_t *q_row(const AttnArgs &a, int first, int h, int r, int node) {
-    return a.q + ((first + node) * a.qrs + (long)(h * a.G + r - node * a.G) * a.qhs) * (F32 ? 4 : 2);
-}
+        const int k2 = f16_exp(max_over_g(m));
+        const float sc = exp2i(k2);
+#pragma unroll
+        for (int k = 0; k < NC; k++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float x = v[k][j][e] * sc;
+                    f[k][j][0][e] = (_Float16)x;
+                    if constexpr (QP == 2) f[k][j][1][e] = (_Float16)(x - (float)(_Float16)x);
+                }
+        return exp2i(-k2) * (scale * 1.4426950408889634f);
+    }
+};
 __device__ __forceinline__ uint64_t node_mask(const AttnArgs &a, int first, int node) {
     return a.tree ? a.tree[first + node] : node == 63 ? ~0ull : (2ull << node) - 1;
 }
@@ -235,10 +244,10 @@ struct Tile {
     float4 ks[2], vs[2];
 };
 
-template <int FMT, int D, int RB, bool F32>
-__global__ void __launch_bounds__(64 * kAttnWaves)
+template <int FMT, int D, int RB, int DT>
+__global__ void __launch_bounds__(64 * kAttnWaves, RB * D <= 256 ? 2 : 1)
 k_tree_attn(KvView c, AttnArgs a) {
-    constexpr int NC = D / 64, NP = F32 ? 2 : 1, ROWS = 16 * RB, LD = D + 4;
+    constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), ROWS = 16 * RB, LD = D + 4;
     __shared__ float s_o[kAttnWaves][ROWS * LD];
     __shared__ float s_m[kAttnWaves][ROWS], s_l[kAttnWaves][ROWS];
     __shared__ int s_ve[kAttnWaves];
@@ -293,30 +302,32 @@ k_tree_attn(KvView c, AttnArgs a) {
 
     // Q: fp16 fragments scaled per row, and what undoes the scaling; the waves
     // share the row blocks out and leave them in LDS, in lane order
-    f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][NP][64]
-    auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * NP + n) << 6) + lane; };
-    Rows<RB, NC, NP> R;
+    f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][QP][64]
+    auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * QP + n) << 6) + lane; };
+    Rows<RB, NC, PP> R;
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
         R.see[rb] = node_mask(a, sr.x, node);
         if ((rb & (kAttnWaves - 1)) != wave) continue;
-        f16x8_t f[NC][2][NP];
-        const float undo = q_frags<NC, NP>(a, q_row<F32>(a, sr.x, h, r, node), g, f);
+        QRow<NC, DT> q;
+        q.load(a, sr.x, h, r, node, g);
+        f16x8_t f[NC][2][QP];
+        const float undo = q.widen(a.scale, f);
         if (g == 0) s_m[0][16 * rb + l16] = undo;
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int n = 0; n < NP; n++) s_q[frag(rb, k, j, n)] = f[k][j][n];
+                for (int n = 0; n < QP; n++) s_q[frag(rb, k, j, n)] = f[k][j][n];
     }
     __syncthreads();
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) R.qs[rb] = s_m[0][16 * rb + l16];
     // up to 32 registers of Q stay there, more are read from LDS tile by tile
-    constexpr bool QREG = RB * NC * 2 * NP * 4 <= 32;
-    f16x8_t qf[QREG ? RB : 1][QREG ? NC : 1][2][NP];
+    constexpr bool QREG = RB * NC * 2 * QP * 4 <= 32;
+    f16x8_t qf[QREG ? RB : 1][QREG ? NC : 1][2][QP];
     if constexpr (QREG) {
 #pragma unroll
         for (int rb = 0; rb < RB; rb++)
@@ -325,7 +336,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int n = 0; n < NP; n++) qf[rb][k][j][n] = s_q[frag(rb, k, j, n)];
+                    for (int n = 0; n < QP; n++) qf[rb][k][j][n] = s_q[frag(rb, k, j, n)];
     }
     auto q_of = [&](int rb, int k, int j, int n, int at) {
         if constexpr (QREG) return qf[rb][k][j][n];
@@ -350,7 +361,7 @@ k_tree_attn(KvView c, AttnArgs a) {
                 f16x8_t ka, kb;
                 codes16<FMT>(w.k[i][k], ka, kb);
 #pragma unroll
-                for (int n = 0; n < NP; n++) {
+                for (int n = 0; n < QP; n++) {
 #pragma unroll
                     for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(ka, q_of(rb, k, 0, n, again), s[rb][i]);
 #pragma unroll
@@ -381,7 +392,7 @@ k_tree_attn(KvView c, AttnArgs a) {
                         for (int q = 0; q < 4; q++) w.v[i][k][q] &= token_bytes(n4[i]);
             }
         }
-        f16x8_t pf[RB][NP];
+        f16x8_t pf[RB][PP];
         R.step(s, vs, pf);
         // results
 #pragma unroll
@@ -398,7 +409,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                 for (int rb = 0; rb < RB; rb++)
 #pragma unroll
-                    for (int n = 0; n < NP; n++) R.o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], R.o[rb][k][q]);
+                    for (int n = 0; n < PP; n++) R.o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], R.o[rb][k][q]);
         }
         t += kAttnWaves;
         if (more) load_v(t, pn);
@@ -456,7 +467,7 @@ k_tree_attn(KvView c, AttnArgs a) {
         const int node = (row0 + r) / a.G, head = h * a.G + (row0 + r) - node * a.G;
         const long t = sr.x + node;
         if (a.splits == 1) {
-            store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, x);
+            store4<DT>(a.out, t * a.ors + head * a.ohs + d, x);
         } else {
             const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
             *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
@@ -473,13 +484,13 @@ k_tree_attn(KvView c, AttnArgs a) {
 // ahead of their use, one barrier a step.
 constexpr int kWideWaves = 8;
 
-template <int FMT, int D, int RB, bool F32, int WT>
+template <int FMT, int D, int RB, int DT, int WT>
 __global__ void __launch_bounds__(64 * kWideWaves)
 k_tree_wide(KvView c, AttnArgs a) {
-    constexpr int NC = D / 64, NP = F32 ? 2 : 1, WR = kWideWaves / WT, ROWS = 16 * RB * WR;
+    constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), WR = kWideWaves / WT, ROWS = 16 * RB * WR;
     constexpr int NF = 8 * NC;                              // fragments a tile: 4 NC of K, then 4 NC of V
     constexpr int UNITS = WT * 4 * NC, UN = (UNITS + kWideWaves - 1) / kWideWaves, LJ = 68;
-    constexpr int TILES = 2 * WT * NF * 64 * 16, JOIN = WT > 1 ? kWideWaves * 16 * RB * LJ * 4 : 0;
+    constexpr int TILES = 2 * WT * NF * 64 * 16, JOIN = kWideWaves * 16 * (WT > 1 ? RB : 1) * LJ * 4;
     __shared__ __attribute__((aligned(16))) uint8_t s_buf[TILES > JOIN ? TILES : JOIN];
     __shared__ float s_sc[2][WT][64];                       // 32 key scales, 32 value scales
     __shared__ float s_m[kWideWaves][16 * RB], s_l[kWideWaves][16 * RB];
@@ -566,6 +577,14 @@ k_tree_wide(KvView c, AttnArgs a) {
         }
         if (wave < WT) s_sc[step & 1][wave][lane] = raw_sc;
     };
+    Rows<RB, NC, PP> R;
+    QRow<NC, DT> q[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        const int r = min(row0 + 16 * (RB * wr + rb) + l16, rows - 1), node = r / a.G;
+        q[rb].load(a, sr.x, h, r, node, g);
+        R.see[rb] = node_mask(a, sr.x, node);
+    }
     int2 pc[WT], pn[WT], pf2[WT];                           // pages of this step's tiles and of the next two
 #pragma unroll
     for (int w = 0; w < WT; w++) {
@@ -574,15 +593,9 @@ k_tree_wide(KvView c, AttnArgs a) {
         pf2[w] = pages(t0 + 2 * WT + w);
     }
     if (steps > 0) request(0, pc);
-
-    Rows<RB, NC, NP> R;
-    f16x8_t qf[RB][NC][2][NP];
+    f16x8_t qf[RB][NC][2][QP];
 #pragma unroll
-    for (int rb = 0; rb < RB; rb++) {
-        const int r = min(row0 + 16 * (RB * wr + rb) + l16, rows - 1), node = r / a.G;
-        R.see[rb] = node_mask(a, sr.x, node);
-        R.qs[rb] = q_frags<NC, NP>(a, q_row<F32>(a, sr.x, h, r, node), g, qf[rb]);
-    }
+    for (int rb = 0; rb < RB; rb++) R.qs[rb] = q[rb].widen(a.scale, qf[rb]);
     R.clear();
     if (steps > 0) widen(0, pc);
     if (steps > 1) request(1, pn);
@@ -607,7 +620,7 @@ k_tree_wide(KvView c, AttnArgs a) {
                     for (int j = 0; j < 2; j++) {
                         const f16x8_t kf = *reinterpret_cast<const f16x8_t *>(buf + ((i * NC + k) * 2 + j) * 1024);
 #pragma unroll
-                        for (int n = 0; n < NP; n++)
+                        for (int n = 0; n < QP; n++)
 #pragma unroll
                             for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(kf, qf[rb][k][j][n], s[rb][i]);
                     }
@@ -630,7 +643,7 @@ k_tree_wide(KvView c, AttnArgs a) {
                 const int node0[2] = {j0[0] - ctx, j0[1] - ctx};
                 R.hide(s, vs, n4, node0);
             }
-            f16x8_t pf[RB][NP];
+            f16x8_t pf[RB][PP];
             R.step(s, vs, pf);
 #pragma unroll
             for (int k = 0; k < NC; k++)
@@ -638,7 +651,7 @@ k_tree_wide(KvView c, AttnArgs a) {
                 for (int q = 0; q < 4; q++) {
                     const f16x8_t vf = *reinterpret_cast<const f16x8_t *>(buf + (4 * NC + 4 * k + q) * 1024);
 #pragma unroll
-                    for (int n = 0; n < NP; n++)
+                    for (int n = 0; n < PP; n++)
 #pragma unroll
                         for (int rb = 0; rb < RB; rb++) R.o[rb][k][q] = mfma_f16(vf, pf[rb][n], R.o[rb][k][q]);
                 }
@@ -652,33 +665,47 @@ k_tree_wide(KvView c, AttnArgs a) {
         __syncthreads();
     }
 
+    // 4 channels of a row, to the results or the workspace; 64 channels of a row
+    // a turn, brought side by side through LDS
     const int heads = c.heads * a.G;
-    auto put = [&](int r, int d, float4 x, float mn, float sum, bool first) {
+    struct Place { long t; int head; size_t at; };
+    auto place = [&](int r) {
         const int node = r / a.G, head = h * a.G + r - node * a.G;
-        const long t = sr.x + node;
-        if (a.splits == 1) {
-            store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, x);
-        } else {
-            const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
-            *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
-            if (first) a.pml[at] = make_float2(mn, sum);
-        }
+        return Place{sr.x + node, head, ((size_t)blockIdx.x * a.T + sr.x + node) * heads + head};
     };
+    auto put = [&](const Place &p, int d, float4 x) {
+        if (a.splits == 1) store4<DT>(a.out, p.t * a.ors + p.head * a.ohs + d, x);
+        else *reinterpret_cast<float4 *>(a.po + p.at * D + d) = x;
+    };
+    float *s_j = reinterpret_cast<float *>(s_buf);          // WT 1: [waves][16][LJ], else [waves][16 RB][LJ]
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) R.l[rb] = sum_over_g(R.l[rb]);
     if constexpr (WT == 1) {
+        if (!live) return;
+        s_j += wave * (16 * LJ);
         const float back = exp2i(R.ve - 6);
 #pragma unroll
         for (int rb = 0; rb < RB; rb++) {
-            const int r = row0 + 16 * (RB * wr + rb) + l16;
+            const int r0 = row0 + 16 * (RB * wr + rb);
             const float inv = R.l[rb] == 0.0f ? 0.0f : back / R.l[rb];
-            if (r < rows)
+            if (a.splits > 1 && g == 0 && r0 + l16 < rows) a.pml[place(r0 + l16).at] = make_float2(R.m[rb], R.l[rb]);
+            Place p[4];
 #pragma unroll
-                for (int k = 0; k < NC; k++)
+            for (int n = 0; n < 4; n++) p[n] = place(min(r0 + 4 * n + g, rows - 1));
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        put(r, 64 * k + 16 * g + 4 * i, make_float4(R.o[rb][k][0][i] * inv, R.o[rb][k][1][i] * inv,
-                            R.o[rb][k][2][i] * inv, R.o[rb][k][3][i] * inv), R.m[rb], R.l[rb], k + g + i == 0);
+            for (int k = 0; k < NC; k++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(&s_j[l16 * LJ + 16 * g + 4 * i]) =
+                        make_float4(R.o[rb][k][0][i] * inv, R.o[rb][k][1][i] * inv, R.o[rb][k][2][i] * inv, R.o[rb][k][3][i] * inv);
+                wave_lds_fence();
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(&s_j[(4 * n + g) * LJ + 4 * l16]);
+                    if (r0 + 4 * n + g < rows) put(p[n], 64 * k + 4 * l16, x);
+                }
+                wave_lds_fence();
+            }
         }
     } else {
 #pragma unroll
@@ -701,7 +728,6 @@ k_tree_wide(KvView c, AttnArgs a) {
             f[rb] = __builtin_amdgcn_exp2f(R.m[rb] - mn) * pow2_ratio(R.ve - vn);
         }
         const float back = exp2i(vn - 6);
-        float *s_j = reinterpret_cast<float *>(s_buf);      // [waves][16 RB][LJ]: 64 channels at a time
 #pragma unroll
         for (int k = 0; k < NC; k++) {
 #pragma unroll
@@ -725,7 +751,9 @@ k_tree_wide(KvView c, AttnArgs a) {
                     sum += s_l[w * WR + rw][rr] * __builtin_amdgcn_exp2f(s_m[w * WR + rw][rr] - mn);
                 }
                 const float inv = sum == 0.0f ? 0.0f : back / sum;
-                put(row0 + r, 64 * k + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv), mn, sum, k + d == 0);
+                const Place p = place(row0 + r);
+                put(p, 64 * k + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+                if (a.splits > 1 && k + d == 0) a.pml[p.at] = make_float2(mn, sum);
             }
             __syncthreads();
         }
@@ -734,7 +762,7 @@ k_tree_wide(KvView c, AttnArgs a) {
 
 // out(t, h) = sum_s w_s o_s / sum_s w_s, w_s = sum_s 2^(max_s - max): one block a
 // row and head, a thread 4 channels of every (1024 / D)-th split.
-template <int D>
+template <int D, int DT>
 __global__ void __launch_bounds__(256)
 k_tree_join(AttnArgs a, int heads) {
     constexpr int TD = D / 4, NG = 256 / TD;
@@ -789,7 +817,48 @@ k_tree_join(AttnArgs a, int heads) {
         x.x += z.x; x.y += z.y; x.z += z.z; x.w += z.w;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store4(a.out, t * a.ors + head * a.ohs + d, a.dtype, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+}
+
+// The same where the splits are few (up to kFewSplits): a thread 4 channels of
+// a row and head over all splits, 1024 / D rows and heads a block.
+constexpr int kFewSplits = 8;
+template <int D, int DT>
+__global__ void __launch_bounds__(256)
+k_tree_join_few(AttnArgs a, int heads) {
+    constexpr int TD = D / 4;
+    const int2 sr = seq_rows(a.row_start, (int)blockIdx.z, a.T, a.max_nodes);
+    const int i = (int)blockIdx.x * (256 / TD) + (int)threadIdx.x / TD, node = i / heads, head = i - node * heads;
+    if (node >= sr.y) return;
+    const int d = (int)threadIdx.x % TD * 4;
+    const long t = sr.x + node;
+    const size_t row = (size_t)t * heads + head, step = (size_t)a.T * heads;
+    float2 ml[kFewSplits];
+    float4 y[kFewSplits];
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) {
+        ml[s] = make_float2(kNoMax, 0.0f);
+        y[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < a.splits) {
+            ml[s] = a.pml[s * step + row];
+            y[s] = *reinterpret_cast<const float4 *>(a.po + (s * step + row) * D + d);
+        }
+    }
+    float mn = kNoMax, sum = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) mn = fmaxf(mn, ml[s].x);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < kFewSplits; s++) {
+        const float w = ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - mn);
+        sum += w;
+        // a split without keys wrote no result
+        const bool none = w == 0.0f;
+        x.x = none ? x.x : fmaf(w, y[s].x, x.x); x.y = none ? x.y : fmaf(w, y[s].y, x.y);
+        x.z = none ? x.z : fmaf(w, y[s].z, x.z); x.w = none ? x.w : fmaf(w, y[s].w, x.w);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
 // How a call is laid out: 16 RB rows a wave; few rows (wt 0) as k_tree_attn, more
@@ -839,27 +908,42 @@ static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
     return splits == 1 ? 0 : (size_t)splits * T * q_heads * (c->head_dim + 2) * 4;
 }
 
-template <int FMT, int D, bool F32>
+template <int FMT, int D, int DT>
 static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, dim3 g, hipStream_t s) {
-    if (p.wt) {
-        constexpr int RB = wide_blocks(D, F32);
-        const dim3 b(64 * kWideWaves);
-        if (p.wt == 1) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, F32, 1>), g, b, 0, s, v, a);
-        else hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, F32, 2>), g, b, 0, s, v, a);
-        return;
-    }
-    constexpr int MOST = few_blocks(D, kFewRows, F32);
-    const dim3 b(64 * kAttnWaves);
-    if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, F32>), g, b, 0, s, v, a);
-    else if constexpr (MOST >= 2) {
-        if (p.rb == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, F32>), g, b, 0, s, v, a);
-        else if constexpr (MOST >= 4) hipLaunchKernelGGL((k_tree_attn<FMT, D, 4, F32>), g, b, 0, s, v, a);
+    constexpr bool F32 = DT == QFM_DT_F32;
+    constexpr int RB = wide_blocks(D, F32), MOST = few_blocks(D, kFewRows, F32);
+    const dim3 b(64 * kAttnWaves), bw(64 * kWideWaves);
+    if (p.wt == 1) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 1>), g, bw, 0, s, v, a);
+    else if (p.wt == 2) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 2>), g, bw, 0, s, v, a);
+    else if (p.wt == 4) {
+        if constexpr (D <= 128) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 4>), g, bw, 0, s, v, a);
+    } else if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, DT>), g, b, 0, s, v, a);
+    else if (p.rb == 2) {
+        if constexpr (MOST >= 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, DT>), g, b, 0, s, v, a);
+    } else {
+        if constexpr (MOST >= 4) hipLaunchKernelGGL((k_tree_attn<FMT, D, 4, DT>), g, b, 0, s, v, a);
     }
 }
-template <int FMT, int D>
-static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, dim3 g, hipStream_t s) {
-    if (a.dtype == QFM_DT_F32) attn_launch<FMT, D, true>(v, a, p, g, s);
-    else attn_launch<FMT, D, false>(v, a, p, g, s);
+template <int D, int DT>
+static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, int fmt, int n_seq, hipStream_t s) {
+    const int rows = a.max_nodes * a.G, heads = v.heads * a.G;
+    const dim3 g((unsigned)a.splits, (unsigned)(v.heads * ((rows + p.block - 1) / p.block)), (unsigned)n_seq);
+    if (fmt == QFM_KV_INT8) attn_launch<QFM_KV_INT8, D, DT>(v, a, p, g, s);
+    else attn_launch<QFM_KV_E4M3, D, DT>(v, a, p, g, s);
+    if (a.splits == 1) return;
+    if (a.splits <= kFewSplits) {
+        const dim3 gj((unsigned)((heads * a.max_nodes + 1024 / D - 1) / (1024 / D)), 1, (unsigned)n_seq);
+        hipLaunchKernelGGL((k_tree_join_few<D, DT>), gj, dim3(256), 0, s, a, heads);
+    } else {
+        const dim3 gj((unsigned)heads, (unsigned)a.max_nodes, (unsigned)n_seq);
+        hipLaunchKernelGGL((k_tree_join<D, DT>), gj, dim3(256), 0, s, a, heads);
+    }
+}
+template <int D>
+static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, int dtype, int fmt, int n_seq, hipStream_t s) {
+    if (dtype == QFM_DT_F32) attn_launch<D, QFM_DT_F32>(v, a, p, fmt, n_seq, s);
+    else if (dtype == QFM_DT_BF16) attn_launch<D, QFM_DT_BF16>(v, a, p, fmt, n_seq, s);
+    else attn_launch<D, QFM_DT_F16>(v, a, p, fmt, n_seq, s);
 }
 
 }  // namespace qfm
@@ -913,24 +997,13 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
         return -1;
     }
     if (T == 0) return 0;
-    AttnArgs a{static_cast<const uint8_t *>(q), static_cast<uint8_t *>(out), dtype, G, T, max_nodes, splits,
+    AttnArgs a{static_cast<const uint8_t *>(q), static_cast<uint8_t *>(out), G, T, max_nodes, splits,
                q_row_stride, q_head_stride, out_row_stride, out_head_stride, row_start, ctx, tree, scale, nullptr, nullptr};
     a.po = static_cast<float *>(ws);
     if (splits > 1) a.pml = reinterpret_cast<float2 *>(a.po + (size_t)splits * T * q_heads * D);
-    const dim3 g((unsigned)splits, (unsigned)(c->kv_heads * ((max_nodes * G + p.block - 1) / p.block)), (unsigned)sq->n_seq);
-    const bool i8 = c->fmt == QFM_KV_INT8;
-    switch (D) {
-        case 64: i8 ? attn_launch<QFM_KV_INT8, 64>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 64>(v, a, p, g, s); break;
-        case 128: i8 ? attn_launch<QFM_KV_INT8, 128>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 128>(v, a, p, g, s); break;
-        default: i8 ? attn_launch<QFM_KV_INT8, 256>(v, a, p, g, s) : attn_launch<QFM_KV_E4M3, 256>(v, a, p, g, s); break;
-    }
-    if (check_launch(who)) return -3;
-    if (splits > 1) {
-        const dim3 gj((unsigned)q_heads, (unsigned)max_nodes, (unsigned)sq->n_seq);
-        if (D == 64) hipLaunchKernelGGL(k_tree_join<64>, gj, dim3(256), 0, s, a, q_heads);
-        else if (D == 128) hipLaunchKernelGGL(k_tree_join<128>, gj, dim3(256), 0, s, a, q_heads);
-        else hipLaunchKernelGGL(k_tree_join<256>, gj, dim3(256), 0, s, a, q_heads);
-    }
+    if (D == 64) attn_launch<64>(v, a, p, dtype, c->fmt, sq->n_seq, s);
+    else if (D == 128) attn_launch<128>(v, a, p, dtype, c->fmt, sq->n_seq, s);
+    else attn_launch<256>(v, a, p, dtype, c->fmt, sq->n_seq, s);
     return check_launch(who) ? -3 : 0;
 }
 

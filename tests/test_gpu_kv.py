@@ -151,6 +151,39 @@ def test_values_at_the_ends_of_the_range(fmt, dt):
     st.destroy()
 
 
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_runs_of_every_length_and_alignment(fmt, D):
+    """Rows whose positions begin and break anywhere: four tokens of a channel share a word of the value codes."""
+    lib, rng, st = qfm.load(), np.random.default_rng(D + fmt), qfm.Stream()
+    page, H, n_seq = 16, 2, 3
+    for trial in range(6):
+        seq, pos, at = [], [], [0] * n_seq
+        while len(seq) < 61 + 5 * trial:
+            s, n = int(rng.integers(0, n_seq)), int(rng.integers(1, 12))
+            at[s] += int(rng.integers(0, 3))
+            if rng.random() < 0.2:
+                seq, pos = seq + [s], pos + [-1]                          # a row between that goes nowhere
+            for i in range(n):
+                seq, pos = seq + [s], pos + [at[s]]
+                at[s] += 1
+        if trial == 5:                                                    # backwards: no row continues another
+            seq, pos = seq[::-1], pos[::-1]
+        T = len(seq)
+        seq, pos = np.array(seq, np.int32), np.array(pos, np.int32)
+        max_pages = -(-max(at) // page)
+        c = _kv.Cache(n_seq * max_pages, page, H, D, fmt, _kv.tables(rng, n_seq, max_pages, n_seq * max_pages), rng)
+        if trial == 4:
+            c.table[1, :] = -1
+        refs = c.upload()
+        k, v = _rows(rng, T, H, D), _rows(rng, T, H, D)
+        v[5], k[9] = np.nan, np.inf
+        _write(lib, c, refs, k, v, T * H * D, H * D, D, "f32", seq, pos, st)
+        c.put(k, v, seq, pos)
+        _same(c)
+    st.destroy()
+
+
 def test_pages_behind_four_gigabytes():
     """Codes whose offset needs more than 32 bits: the last pages of a pool of 4.4e9 bytes."""
     lib, rng, st = qfm.load(), np.random.default_rng(3), qfm.Stream()
