@@ -293,27 +293,30 @@ k_tree_attn(KvView c, AttnArgs a) {
             w.vs[i] = *reinterpret_cast<const float4 *>(c.vs + at + 4 * g);
         }
     };
+    // Q: the waves share the row blocks out and leave their fragments in LDS; up to
+    // 32 registers of them are then kept, more are read again tile by tile
+    constexpr bool QREG = RB * NC * 2 * QP * 4 <= 32;
+    f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][QP][64], in lane order
+    auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * QP + n) << 6) + lane; };
+    Rows<RB, NC, PP> R;
+    QRow<NC, DT> q[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; rb++) {
+        const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
+        if ((rb & (kAttnWaves - 1)) == wave) q[rb].load(a, sr.x, h, r, node, g);
+        R.see[rb] = node_mask(a, sr.x, node);
+    }
     int2 pg = pages(t);
     if (t < t1) {
         load_k(t, pg);
         load_v(t, pg);
     }
     int2 pn = pages(t + kAttnWaves);
-
-    // Q: fp16 fragments scaled per row, and what undoes the scaling; the waves
-    // share the row blocks out and leave them in LDS, in lane order
-    f16x8_t *s_q = reinterpret_cast<f16x8_t *>(&s_o[0][0]);        // [RB][NC][2][QP][64]
-    auto frag = [&](int rb, int k, int j, int n) { return ((((rb * NC + k) * 2 + j) * QP + n) << 6) + lane; };
-    Rows<RB, NC, PP> R;
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
-        const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
-        R.see[rb] = node_mask(a, sr.x, node);
         if ((rb & (kAttnWaves - 1)) != wave) continue;
-        QRow<NC, DT> q;
-        q.load(a, sr.x, h, r, node, g);
         f16x8_t f[NC][2][QP];
-        const float undo = q.widen(a.scale, f);
+        const float undo = q[rb].widen(a.scale, f);
         if (g == 0) s_m[0][16 * rb + l16] = undo;
 #pragma unroll
         for (int k = 0; k < NC; k++)
@@ -323,14 +326,11 @@ k_tree_attn(KvView c, AttnArgs a) {
                 for (int n = 0; n < QP; n++) s_q[frag(rb, k, j, n)] = f[k][j][n];
     }
     __syncthreads();
-#pragma unroll
-    for (int rb = 0; rb < RB; rb++) R.qs[rb] = s_m[0][16 * rb + l16];
-    // up to 32 registers of Q stay there, more are read from LDS tile by tile
-    constexpr bool QREG = RB * NC * 2 * QP * 4 <= 32;
     f16x8_t qf[QREG ? RB : 1][QREG ? NC : 1][2][QP];
-    if constexpr (QREG) {
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++)
+    for (int rb = 0; rb < RB; rb++) {
+        R.qs[rb] = s_m[0][16 * rb + l16];
+        if constexpr (QREG)
 #pragma unroll
             for (int k = 0; k < NC; k++)
 #pragma unroll
