@@ -50,45 +50,113 @@ __device__ __forceinline__ int next_slot(int e, uint32_t &left) {
 
 constexpr int kLoraInWaves = 8;
 
-// One 16-row tile of A a workgroup (blockIdx.y over the n projections' tiles);
-// the waves take the chunks of 64 inner values in turn.
-template <int DT, bool EACH>
+// RT 16-row tiles of A a workgroup (blockIdx.y over the n projections' tiles)
+// against CB 16-row blocks of x; the waves take the chunks of 64 inner values in
+// turn, their sums meet in LDS. Rows of A and x lie K apart, so a fragment read
+// straight from memory would take a cache line a lane (2050 rows: 27.6 us); a
+// wave reads 8 rows of 128 bytes a request instead, U chunks together, and turns
+// them in an LDS area of its own.
+template <int DT, int RT, int CB>
 __global__ void __launch_bounds__(64 * kLoraInWaves)
 k_lora_in(LoraArgs a) {
-    __shared__ f32x4_t s_acc[kLoraInWaves][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
-    const int tiles = (a.R + 15) >> 4, i = (int)blockIdx.y / tiles, r0 = ((int)blockIdx.y - i * tiles) * 16;
-    const int e = lora_slot(a, (int)blockIdx.x, l16);
-    uint32_t left = (uint32_t)__ballot(e >= 0) & 0xFFFFu;
-    int skip = EACH ? (int)blockIdx.z : 0;
-    const uint16_t *x = static_cast<const uint16_t *>(a.x) + (size_t)min(16 * (int)blockIdx.x + l16, a.T - 1) * a.xs + 16 * g;
-    while (left) {
-        const int cur = next_slot(e, left);
-        if (EACH && skip--) continue;
-        const uint16_t *w = static_cast<const uint16_t *>(a.a[i]) + ((size_t)cur * a.R + min(r0 + l16, a.R - 1)) * a.K + 16 * g;
-        f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 64 * wave; k < a.K; k += 64 * kLoraInWaves) {
-            const u32x4_t *wp = reinterpret_cast<const u32x4_t *>(w + k), *xp = reinterpret_cast<const u32x4_t *>(x + k);
-            acc = lora_mfma<DT>(wp[0], xp[0], acc);
-            acc = lora_mfma<DT>(wp[1], xp[1], acc);
-        }
-        s_acc[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0) {
+    constexpr int U = RT * CB > 1 ? 2 : 4, NA = 2 * RT, NX = 2 * CB, PART = (NA + NX) * 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[kLoraInWaves * (PART > RT * CB * 1024 ? PART : RT * CB * 1024)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
+    const int l8 = lane >> 3, ch = lane & 7, tiles = (a.R + 15) >> 4, most = a.n * tiles - 1;
+    uint8_t *s_w = s_buf + wave * PART, *s_x = s_w + NA * 1024;
+    f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(s_buf);             // [waves][RT CB][64], once the chunks are done
+    int e[CB];
+    uint32_t left[CB], some = 0;
 #pragma unroll
-            for (int v = 1; v < kLoraInWaves; v++) acc += s_acc[v][lane];
-            const int rank = a.rank[cur];
-            const int r = r0 + 4 * g;
-            if (e == cur && r < a.R) {
-                float4 o = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (r + 0 >= rank) o.x = 0.0f;
-                if (r + 1 >= rank) o.y = 0.0f;
-                if (r + 2 >= rank) o.z = 0.0f;
-                if (r + 3 >= rank) o.w = 0.0f;
-                *reinterpret_cast<float4 *>(a.h + (size_t)(16 * (int)blockIdx.x + l16) * (a.n * a.R) + i * a.R + r) = o;
+    for (int c = 0; c < CB; c++) {
+        e[c] = lora_slot(a, (int)blockIdx.x * CB + c, l16);
+        left[c] = (uint32_t)__ballot(e[c] >= 0) & 0xFFFFu;
+        some |= left[c];
+    }
+    const uint16_t *x[NX];
+#pragma unroll
+    for (int n = 0; n < NX; n++)
+        x[n] = static_cast<const uint16_t *>(a.x) + (size_t)min(16 * CB * (int)blockIdx.x + 8 * n + l8, a.T - 1) * a.xs + 8 * ch;
+    // the adapters of these rows, every gridDim.z-th of them here
+    for (int pass = 0; some; pass++) {
+        // the next adapter: the first left block's first left row has it
+        int cur = -1;
+#pragma unroll
+        for (int c = 0; c < CB; c++)
+            if (cur < 0 && left[c]) cur = __builtin_amdgcn_readlane(e[c], __builtin_ctz(left[c]));
+        some = 0;
+#pragma unroll
+        for (int c = 0; c < CB; c++) {
+            left[c] &= ~(uint32_t)__ballot(e[c] == cur);
+            some |= left[c];
+        }
+        if (pass % (int)gridDim.z != (int)blockIdx.z) continue;
+        const uint16_t *w[NA];
+#pragma unroll
+        for (int n = 0; n < NA; n++) {
+            const int y = min((int)blockIdx.y * RT + n / 2, most), i = y / tiles, r = (y - i * tiles) * 16 + (n & 1) * 8 + l8;
+            w[n] = static_cast<const uint16_t *>(a.a[i]) + ((size_t)cur * a.R + min(r, a.R - 1)) * a.K + 8 * ch;
+        }
+        f32x4_t acc[RT][CB];
+#pragma unroll
+        for (int q = 0; q < RT; q++)
+#pragma unroll
+            for (int c = 0; c < CB; c++) acc[q][c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        const int chunks = a.K / 64;
+        for (int k0 = wave; k0 < chunks; k0 += U * kLoraInWaves) {
+            u32x4_t wv[U][NA], xv[U][NX];
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                const size_t at = 64 * (size_t)min(k0 + v * kLoraInWaves, chunks - 1);
+#pragma unroll
+                for (int n = 0; n < NA; n++) wv[v][n] = *reinterpret_cast<const u32x4_t *>(w[n] + at);
+#pragma unroll
+                for (int n = 0; n < NX; n++) xv[v][n] = *reinterpret_cast<const u32x4_t *>(x[n] + at);
+            }
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                if (k0 + v * kLoraInWaves >= chunks) break;
+#pragma unroll
+                for (int n = 0; n < NA; n++) *reinterpret_cast<u32x4_t *>(s_w + lds_at<128>(8 * n + l8, ch)) = wv[v][n];
+#pragma unroll
+                for (int n = 0; n < NX; n++) *reinterpret_cast<u32x4_t *>(s_x + lds_at<128>(8 * n + l8, ch)) = xv[v][n];
+                wave_lds_fence();
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    u32x4_t xf[CB];
+#pragma unroll
+                    for (int c = 0; c < CB; c++) xf[c] = *reinterpret_cast<const u32x4_t *>(s_x + lds_at<128>(16 * c + l16, 4 * j + g));
+#pragma unroll
+                    for (int q = 0; q < RT; q++) {
+                        const u32x4_t wf = *reinterpret_cast<const u32x4_t *>(s_w + lds_at<128>(16 * q + l16, 4 * j + g));
+#pragma unroll
+                        for (int c = 0; c < CB; c++) acc[q][c] = lora_mfma<DT>(wf, xf[c], acc[q][c]);
+                    }
+                }
+                wave_lds_fence();
             }
         }
-        if (EACH) return;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < RT; q++)
+#pragma unroll
+            for (int c = 0; c < CB; c++) s_acc[(wave * RT * CB + q * CB + c) * 64 + lane] = acc[q][c];
+        const int rank = a.rank[cur];
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < RT * CB; p++) {
+            if (p % kLoraInWaves != wave) continue;
+            f32x4_t sum = s_acc[p * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < kLoraInWaves; v++) sum += s_acc[(v * RT * CB + p) * 64 + lane];
+            const int q = p / CB, c = p % CB, y = (int)blockIdx.y * RT + q, i = y / tiles, r = (y - i * tiles) * 16 + 4 * g;
+            if (y <= most && e[c] == cur && r < a.R) {
+                const float4 o = make_float4(r + 0 < rank ? sum[0] : 0.0f, r + 1 < rank ? sum[1] : 0.0f,
+                                             r + 2 < rank ? sum[2] : 0.0f, r + 3 < rank ? sum[3] : 0.0f);
+                const size_t t = 16 * (size_t)((int)blockIdx.x * CB + c) + l16;
+                *reinterpret_cast<float4 *>(a.h + t * (a.n * a.R) + i * a.R + r) = o;
+            }
+        }
         __syncthreads();
     }
 }
@@ -96,115 +164,172 @@ k_lora_in(LoraArgs a) {
 constexpr int kLoraOutWaves = 4, kLoraOutTiles = 4;   // tiles of 16 outputs a wave
 
 // blockIdx.y: 256 outputs of one projection (first: the projections' first such
-// block). KS: 32-value steps of the rank.
+// block), NB 16-row blocks one after another, so many that all workgroups run
+// at once (a workgroup's first block takes 12 us of 2050 rows' 40, the others 4). B's fragments stay in registers
+// from block to block while the adapter is the same. KS: 32-value steps of the
+// rank.
 struct LoraFirst { int v[5]; };
 template <int DT, int KS, bool EACH>
 __global__ void __launch_bounds__(64 * kLoraOutWaves)
-k_lora_out(LoraArgs a, LoraFirst first) {
+k_lora_out(LoraArgs a, LoraFirst first, int NB) {
     constexpr int NP = DT == QFM_DT_BF16 ? 3 : 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
     int i = 0;
     while (i < 3 && (int)blockIdx.y >= first.v[i + 1]) i++;
     const int N = a.rows[i], o0 = (((int)blockIdx.y - first.v[i]) * kLoraOutWaves + wave) * (16 * kLoraOutTiles);
-    const int t = 16 * (int)blockIdx.x + l16, e = lora_slot(a, (int)blockIdx.x, l16);
-    uint32_t left = (uint32_t)__ballot(e >= 0) & 0xFFFFu;
-    int skip = EACH ? (int)blockIdx.z : 0;
-    bool mine = t < a.T && (EACH ? e < 0 && skip == 0 : true);      // columns that this wave writes
-    f32x4_t acc[kLoraOutTiles];
-#pragma unroll
-    for (int q = 0; q < kLoraOutTiles; q++) acc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float factor = 0.0f;
-    while (left) {
-        const int cur = next_slot(e, left);
-        if (EACH && skip--) continue;
-        const bool here = e == cur;
-        if (EACH) mine |= here;
-        // this row's inner values, whole, as 16-bit numbers
-        float v[KS][8], m = 0.0f;
+    constexpr int LJ = 68;
+    __shared__ __attribute__((aligned(16))) float s_y[kLoraOutWaves][16 * LJ];
+    const bool whole = N % 4 == 0;
+    const float *base0 = a.base[i];
+    const int oc = o0 + 4 * l16;                            // this lane's outputs of rows 4 q + g
+    u32x4_t bf[kLoraOutTiles][KS];
+    int have = -1;                                          // the adapter in bf
+    // a block's slots, inner values and base (4 rows of 256 bytes a request) are
+    // requested a block ahead
+    auto request = [&](int blk, int &e, f32x4_t (&h)[KS][2], f32x4_t (&bs)[4]) {
+        e = lora_slot(a, blk, l16);
+        const float *hp = a.h + (size_t)min(16 * blk + l16, a.T - 1) * (a.n * a.R) + i * a.R;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
+            const f32x4_t *p = reinterpret_cast<const f32x4_t *>(hp + min(32 * s + 8 * g, a.R - 8));
+            h[s][0] = p[0];
+            h[s][1] = p[1];
+        }
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
-            if (here && 32 * s + 8 * g < a.R) {
-                const float4 *p = reinterpret_cast<const float4 *>(a.h + (size_t)t * (a.n * a.R) + i * a.R + 32 * s + 8 * g);
-                const float4 c = p[0], d = p[1];
-                v[s][0] = c.x; v[s][1] = c.y; v[s][2] = c.z; v[s][3] = c.w; v[s][4] = d.x; v[s][5] = d.y; v[s][6] = d.z; v[s][7] = d.w;
+        for (int q = 0; q < 4; q++) {
+            const int tr = 16 * blk + 4 * q + g;
+            bs[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            if (base0 && tr < a.T && oc < N) {
+                const float *p = base0 + (size_t)tr * N + oc;
+                if (whole) bs[q] = *reinterpret_cast<const f32x4_t *>(p);
+                else bs[q] = f32x4_t{p[0], oc + 1 < N ? p[1] : 0.0f, oc + 2 < N ? p[2] : 0.0f, oc + 3 < N ? p[3] : 0.0f};
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[s][j]));
         }
-        float sc = 1.0f, back = 1.0f;
-        if constexpr (DT == QFM_DT_F16) {
-            m = fmaxf(m, __shfl_xor(m, 16));
-            const int k = f16_exp(fmaxf(m, __shfl_xor(m, 32)));
-            sc = exp2i(k);
-            back = exp2i(-k);
-        }
-        u32x4_t hp[KS][NP];
+    };
+    int e, en;
+    f32x4_t h[KS][2], hn[KS][2], bs[4], bn[4];
+    request((int)blockIdx.x * NB, e, h, bs);
+    for (int nb = 0; nb < NB; nb++) {
+        const int blk = (int)blockIdx.x * NB + nb, t = 16 * blk + l16;
+        if (16 * blk >= a.T) return;
+        if constexpr (!EACH) request(min(blk + 1, (a.T - 1) / 16), en, hn, bn);
+        uint32_t left = (uint32_t)__ballot(e >= 0) & 0xFFFFu;
+        int skip = EACH ? (int)blockIdx.z : 0;
+        bool mine = t < a.T && (EACH ? e < 0 && skip == 0 : true);      // rows that this wave writes
+        f32x4_t acc[kLoraOutTiles];
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int q = 0; q < kLoraOutTiles; q++) acc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float factor = 0.0f;
+        while (left) {
+            const int cur = next_slot(e, left);
+            if (EACH && skip--) continue;
+            const bool here = e == cur;
+            if (EACH) mine |= here;
+            if (cur != have) {
+                have = cur;
+                const int rank = min(max(a.rank[cur], 0), a.R);
+                const uint16_t *w = static_cast<const uint16_t *>(a.b[i]) + (size_t)cur * N * a.R;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float c = v[s][2 * j] * sc, d = v[s][2 * j + 1] * sc;
+                for (int q = 0; q < kLoraOutTiles; q++) {
+                    const uint16_t *wr = w + (size_t)min(o0 + 16 * q + l16, N - 1) * a.R;
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    if constexpr (DT == QFM_DT_BF16) {
-                        const uint32_t u = (uint32_t)f32_to_bf16(c) | ((uint32_t)f32_to_bf16(d) << 16);
-                        hp[s][p][j] = u;
-                        c -= bf16_lo(u);
-                        d -= bf16_hi(u);
-                    } else {
-                        const f16x2_t u = {(_Float16)c, (_Float16)d};
-                        hp[s][p][j] = __builtin_bit_cast(uint32_t, u);
-                        c -= (float)u.x;
-                        d -= (float)u.y;
+                    for (int s = 0; s < KS; s++) {
+                        const int k = 32 * s + 8 * g, keep = rank - k;  // columns from rank on count as zeros
+                        u32x4_t b = *reinterpret_cast<const u32x4_t *>(wr + min(k, a.R - 8));
+#pragma unroll
+                        for (int j = 0; j < 4; j++) b[j] &= keep >= 2 * j + 2 ? ~0u : keep == 2 * j + 1 ? 0xFFFFu : 0u;
+                        bf[q][s] = b;
                     }
                 }
             }
-        const int rank = min(max(a.rank[cur], 0), a.R);
-        if (here) factor = a.scale[cur] * back;
-        const uint16_t *w = static_cast<const uint16_t *>(a.b[i]) + (size_t)cur * N * a.R;
-#pragma unroll
-        for (int q = 0; q < kLoraOutTiles; q++) {
-            const uint16_t *wr = w + (size_t)min(o0 + 16 * q + l16, N - 1) * a.R;
-            f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+            // this row's inner values, whole, as 16-bit numbers
+            float v[KS][8], m = 0.0f;
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                const int k = 32 * s + 8 * g, keep = rank - k;      // columns from rank on count as zeros
-                u32x4_t b = {0u, 0u, 0u, 0u};
-                if (keep > 0) b = *reinterpret_cast<const u32x4_t *>(wr + k);
-                if (keep < 8) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) b[j] &= keep >= 2 * j + 2 ? ~0u : keep == 2 * j + 1 ? 0xFFFFu : 0u;
+                for (int j = 0; j < 8; j++) v[s][j] = 0.0f;
+                if (here && 32 * s + 8 * g < a.R) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[s][j] = h[s][j / 4][j % 4];
                 }
 #pragma unroll
-                for (int p = 0; p < NP; p++) sum = lora_mfma<DT>(b, hp[s][p], sum);
+                for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[s][j]));
             }
-            // chosen, not added: an infinite weight times another row's zeros is NaN
+            float sc = 1.0f, back = 1.0f;
+            if constexpr (DT == QFM_DT_F16) {
+                m = fmaxf(m, __shfl_xor(m, 16));
+                const int k = f16_exp(fmaxf(m, __shfl_xor(m, 32)));
+                sc = exp2i(k);
+                back = exp2i(-k);
+            }
+            u32x4_t hp[KS][NP];
 #pragma unroll
-            for (int j = 0; j < 4; j++) acc[q][j] = here ? sum[j] : acc[q][j];
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    float c = v[s][2 * j] * sc, d = v[s][2 * j + 1] * sc;
+#pragma unroll
+                    for (int p = 0; p < NP; p++) {
+                        if constexpr (DT == QFM_DT_BF16) {
+                            // cut off after 8 bits, three times: 24 bits, nothing lost
+                            const uint32_t u = pack_bf16_hi(c, d);
+                            hp[s][p][j] = u;
+                            c -= bf16_lo(u);
+                            d -= bf16_hi(u);
+                        } else {
+                            const f16x2_t u = {(_Float16)c, (_Float16)d};
+                            hp[s][p][j] = __builtin_bit_cast(uint32_t, u);
+                            c -= (float)u.x;
+                            d -= (float)u.y;
+                        }
+                    }
+                }
+            if (here) factor = a.scale[cur] * back;
+#pragma unroll
+            for (int q = 0; q < kLoraOutTiles; q++) {
+                f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int p = 0; p < NP; p++) sum = lora_mfma<DT>(bf[q][s], hp[s][p], sum);
+                // chosen, not added: an infinite weight times another row's zeros is NaN
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[q][j] = here ? sum[j] : acc[q][j];
+            }
+            if (EACH) break;
         }
-        if (EACH) break;
-    }
-    if (!mine) return;
-    const bool whole = N % 4 == 0;
+        const uint32_t rows = (uint32_t)__ballot(mine) & 0xFFFFu;
+        float *sy = s_y[wave];
 #pragma unroll
-    for (int q = 0; q < kLoraOutTiles; q++) {
-        const int o = o0 + 16 * q + 4 * g;
-        if (o >= N) break;
-        const size_t at = (size_t)t * N + o;
-        float *y = a.y[i] + at;
-        const float *base = a.base[i] ? a.base[i] + at : nullptr;
-        if (whole) {
-            float4 v = base ? *reinterpret_cast<const float4 *>(base) : make_float4(0.f, 0.f, 0.f, 0.f);
-            v.x = fmaf(factor, acc[q][0], v.x); v.y = fmaf(factor, acc[q][1], v.y);
-            v.z = fmaf(factor, acc[q][2], v.z); v.w = fmaf(factor, acc[q][3], v.w);
-            *reinterpret_cast<float4 *>(y) = v;
-        } else {
+        for (int q = 0; q < kLoraOutTiles; q++)
+            *reinterpret_cast<float4 *>(&sy[l16 * LJ + 16 * q + 4 * g]) =
+                make_float4(factor * acc[q][0], factor * acc[q][1], factor * acc[q][2], factor * acc[q][3]);
+        wave_lds_fence();
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (o + j < N) y[j] = fmaf(factor, acc[q][j], base ? base[j] : 0.0f);
+        for (int q = 0; q < 4; q++) {
+            const float4 d = *reinterpret_cast<const float4 *>(&sy[(4 * q + g) * LJ + 4 * l16]);
+            if (!(rows >> (4 * q + g) & 1) || oc >= N) continue;
+            const float4 v = make_float4(bs[q][0] + d.x, bs[q][1] + d.y, bs[q][2] + d.z, bs[q][3] + d.w);
+            float *y = a.y[i] + (size_t)(16 * blk + 4 * q + g) * N + oc;
+            if (whole) {
+                *reinterpret_cast<float4 *>(y) = v;
+            } else {
+                y[0] = v.x;
+                if (oc + 1 < N) y[1] = v.y;
+                if (oc + 2 < N) y[2] = v.z;
+                if (oc + 3 < N) y[3] = v.w;
+            }
         }
+        wave_lds_fence();
+        if constexpr (EACH) return;
+        e = en;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            h[s][0] = hn[s][0];
+            h[s][1] = hn[s][1];
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) bs[q] = bn[q];
     }
 }
 
@@ -224,12 +349,15 @@ static int lora_check(const qfm_lora *l, int T, const char *who) {
 
 template <int DT, bool EACH>
 static void lora_launch(const LoraArgs &a, const LoraFirst &f, hipStream_t s) {
-    const unsigned blocks = (unsigned)((a.T + 15) / 16), z = EACH ? 16u : 1u;
-    hipLaunchKernelGGL((k_lora_in<DT, EACH>), dim3(blocks, (unsigned)(a.n * ((a.R + 15) / 16)), z), dim3(64 * kLoraInWaves), 0, s, a);
-    const dim3 g(blocks, (unsigned)f.v[4], z), b(64 * kLoraOutWaves);
-    if (a.R <= 32) hipLaunchKernelGGL((k_lora_out<DT, 1, EACH>), g, b, 0, s, a, f);
-    else if (a.R <= 64) hipLaunchKernelGGL((k_lora_out<DT, 2, EACH>), g, b, 0, s, a, f);
-    else hipLaunchKernelGGL((k_lora_out<DT, 4, EACH>), g, b, 0, s, a, f);
+    constexpr int RT = EACH ? 1 : 4, CB = EACH ? 1 : 2;
+    const int blocks = (a.T + 15) / 16, tiles = a.n * ((a.R + 15) / 16);
+    hipLaunchKernelGGL((k_lora_in<DT, RT, CB>), dim3((unsigned)((blocks + CB - 1) / CB), (unsigned)((tiles + RT - 1) / RT), EACH ? 16u : 4u),
+                       dim3(64 * kLoraInWaves), 0, s, a);
+    const int nb = EACH ? 1 : (int)(((long)blocks * f.v[4] + 511) / 512);
+    const dim3 g((unsigned)((blocks + nb - 1) / nb), (unsigned)f.v[4], EACH ? 16u : 1u), b(64 * kLoraOutWaves);
+    if (a.R <= 32) hipLaunchKernelGGL((k_lora_out<DT, 1, EACH>), g, b, 0, s, a, f, nb);
+    else if (a.R <= 64) hipLaunchKernelGGL((k_lora_out<DT, 2, EACH>), g, b, 0, s, a, f, nb);
+    else hipLaunchKernelGGL((k_lora_out<DT, 4, EACH>), g, b, 0, s, a, f, nb);
 }
 
 }  // namespace qfm
