@@ -56,8 +56,8 @@ __device__ __forceinline__ void load_row(const uint8_t *p, float (&v)[VL]) {
     }
 }
 
-// codes (VL / 4 words) and scale of this lane's part of a row; 16 lanes a row
-template <int FMT, int VL>
+// codes (VL / 4 words) and scale of this lane's part of a row; LPR lanes a row
+template <int FMT, int VL, int LPR>
 __device__ __forceinline__ float quantise(const float (&v)[VL], uint32_t (&code)[VL / 4]) {
     constexpr float kInv = FMT == QFM_KV_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
     // the largest magnitude as bits: NaN and infinity above every number
@@ -65,7 +65,7 @@ __device__ __forceinline__ float quantise(const float (&v)[VL], uint32_t (&code)
 #pragma unroll
     for (int i = 0; i < VL; i++) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
 #pragma unroll
-    for (int o = 8; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
+    for (int o = LPR / 2; o; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
     const bool fine = m < 0x7F800000u;
     float s = __uint_as_float(m) * kInv;
     if (s == 0.0f) s = 1.0f;
@@ -96,13 +96,41 @@ __device__ __forceinline__ uint32_t transpose_rows(uint32_t x, int r) {
     return r & 2 ? __builtin_amdgcn_perm(z, w, 0x07060302u) : __builtin_amdgcn_perm(w, z, 0x05040100u);
 }
 
+// Few rows (up to kFewRows): what counts is the chain row -> place -> stores, so
+// keys and values are rows of their own, 8 values a lane, every value code a byte
+// store (8 rows of 2 x 256: 4.4 us a call, 5.4 in fours as below).
+constexpr int kFewRows = 64;
+template <int DT, int FMT, int D>
+__global__ void __launch_bounds__(kKvThreads)
+k_kv_write_few(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ v, long rs, long hs,
+               const int *__restrict__ seq, const int *__restrict__ pos, int T) {
+    constexpr int LPR = D / 8, ES = DT == QFM_DT_F32 ? 4 : 2;
+    const int u = ((int)blockIdx.x * kKvThreads + (int)threadIdx.x) / LPR, j = (int)threadIdx.x % LPR, kv = u & 1;
+    const int t = (u >> 1) / c.heads, h = (u >> 1) - t * c.heads;
+    if (t >= T) return;                                     // whole rows: LPR lanes leave together
+    float x[8];
+    load8<DT>((kv ? v : k) + (t * rs + h * hs + 8 * j) * ES, x);
+    const int sq = seq[t], p = pos[t];
+    const int page = (unsigned)sq < (unsigned)c.n_seq ? c.page_of(sq, p) : -1;
+    const int tok = p & (c.page() - 1);
+    uint32_t code[2];
+    const float s = quantise<FMT, 8, LPR>(x, code);
+    if (page < 0) return;
+    const size_t at = c.token0(page, h);
+    if (j == 0) (kv ? c.vs : c.ks)[at + tok] = s;
+    if (kv) {
+        uint8_t *o = c.v + (at + (tok & ~3)) * D + (8 * j) * 4 + (tok & 3);
+#pragma unroll
+        for (int q = 0; q < 8; q++) o[4 * q] = (uint8_t)(code[q / 4] >> (8 * (q % 4)));
+    } else {
+        *reinterpret_cast<uint2 *>(c.k + (at + tok) * D + 8 * j) = make_uint2(code[0], code[1]);
+    }
+}
+
 // One wave takes 4 rows of a head, 16 lanes a row. Keys go as they are. Values
 // lie four tokens to a word: where 4 rows in a row fill such a word (positions 4
 // n .. 4 n + 3 of one sequence) the wave in whose rows the first one is takes
-// those four and writes words; the other rows' values go byte by byte. Up to
-// kByteRows rows all do: what counts there is the chain of loads, which the
-// fours make longer (8 rows: 4.4 us a call, 5.4 with them).
-constexpr int kByteRows = 64;
+// those four and writes words; the other rows' values go byte by byte.
 template <int DT, int FMT, int D>
 __global__ void __launch_bounds__(kKvThreads)
 k_kv_write(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ v, long rs, long hs,
@@ -114,17 +142,14 @@ k_kv_write(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ 
     if (b >= T) return;
     const uint8_t *kp = k + (h * hs + VL * j) * ES, *vp = v + (h * hs + VL * j) * ES;
     const int t = min(b + r, T - 1);
-    const bool words = T > kByteRows;
     float x[VL], y[VL];
     load_row<DT, VL>(kp + (long)t * rs * ES, x);
-    if (!words) load_row<DT, VL>(vp + (long)t * rs * ES, y);
     // rows b - 3 .. b + 12: which continue their predecessor's sequence
     const int ti = b - 3 + j;
     const int ts = ti >= 0 && ti < T ? seq[ti] : -1, tp = ti >= 0 && ti < T ? pos[ti] : -1;
     const int bs = __shfl(ts, j - 1), bp = __shfl(tp, j - 1);                  // (every lane takes part)
     const uint32_t cont = (uint32_t)__ballot(j > 0 && tp > 0 && ts == bs && tp == bp + 1) & 0xFFFFu;   // bit j: row b - 3 + j
-    const uint32_t four = (uint32_t)__ballot(tp >= 0 && (tp & 3) == 0) & 0xFFFFu & cont >> 1 & cont >> 2 & cont >> 3;
-    const uint32_t first = words ? four : 0u;
+    const uint32_t first = (uint32_t)__ballot(tp >= 0 && (tp & 3) == 0) & 0xFFFFu & cont >> 1 & cont >> 2 & cont >> 3;
     // first: rows that begin four in a row; the one among this wave's own, if any
     const uint32_t mine = first >> 3 & 0xFu;
     const int q0 = mine ? __builtin_ctz(mine) : 0;
@@ -133,8 +158,8 @@ k_kv_write(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ 
     const int page = b + r < T && (unsigned)sq < (unsigned)c.n_seq ? c.page_of(sq, p) : -1;
     const int tok = p & (c.page() - 1);
     uint32_t code[VL / 4];
-    float s = quantise<FMT, VL>(x, code);
-    if (words) load_row<DT, VL>(vp + (long)(mine ? min(b + q0 + r, T - 1) : t) * rs * ES, y);
+    float s = quantise<FMT, VL, 16>(x, code);
+    load_row<DT, VL>(vp + (long)(mine ? min(b + q0 + r, T - 1) : t) * rs * ES, y);
     if (page >= 0) {
         const size_t at = c.token0(page, h) + tok;
         uint32_t *o = reinterpret_cast<uint32_t *>(c.k + at * D + VL * j);
@@ -143,7 +168,7 @@ k_kv_write(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ 
         if (j == 0) c.ks[at] = s;
     }
     if (mine) {
-        s = quantise<FMT, VL>(y, code);
+        s = quantise<FMT, VL, 16>(y, code);
         const int qs = __shfl(ts, q0 + 3), qp = __shfl(tp, q0 + 3);
         const int pg = (unsigned)qs < (unsigned)c.n_seq ? c.page_of(qs, qp) : -1;
         const size_t at = c.token0(max(pg, 0), h) + (qp & (c.page() - 1));
@@ -159,7 +184,7 @@ k_kv_write(KvView c, const uint8_t *__restrict__ k, const uint8_t *__restrict__ 
     const bool single = page >= 0 && !(part >> (3 + r) & 1);
     if (!__any(single)) return;
     if (mine) load_row<DT, VL>(vp + (long)t * rs * ES, y);
-    s = quantise<FMT, VL>(y, code);
+    s = quantise<FMT, VL, 16>(y, code);
     if (!single) return;
     const size_t at = c.token0(page, h);
     uint8_t *o = c.v + (at + (tok & ~3)) * D + VL * j * 4 + (tok & 3);
@@ -291,7 +316,12 @@ int qfm_kv_write(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *k, co
     const long waves = (long)((T + 3) / 4) * w.heads;
     const dim3 g((unsigned)((waves + kKvThreads / 64 - 1) / (kKvThreads / 64))), b(kKvThreads);
 #define QFM_KV_ARGS w, static_cast<const uint8_t *>(k), static_cast<const uint8_t *>(v), row_stride, head_stride, seq, pos, T
-    QFM_KV_LAUNCH(k_kv_write)
+    if (T <= kFewRows) {
+        const dim3 g((unsigned)((T * w.heads * 2 * (c->head_dim / 8) + kKvThreads - 1) / kKvThreads));
+        QFM_KV_LAUNCH(k_kv_write_few)
+    } else {
+        QFM_KV_LAUNCH(k_kv_write)
+    }
 #undef QFM_KV_ARGS
     return check_launch(who) ? -3 : 0;
 }

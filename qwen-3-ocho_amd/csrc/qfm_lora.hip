@@ -351,7 +351,7 @@ template <int DT, bool EACH>
 static void lora_launch(const LoraArgs &a, const LoraFirst &f, hipStream_t s) {
     constexpr int RT = EACH ? 1 : 4, CB = EACH ? 1 : 2;
     const int blocks = (a.T + 15) / 16, tiles = a.n * ((a.R + 15) / 16);
-    hipLaunchKernelGGL((k_lora_in<DT, RT, CB>), dim3((unsigned)((blocks + CB - 1) / CB), (unsigned)((tiles + RT - 1) / RT), EACH ? 16u : 4u),
+    hipLaunchKernelGGL((k_lora_in<DT, RT, CB>), dim3((unsigned)((blocks + CB - 1) / CB), (unsigned)((tiles + RT - 1) / RT), EACH ? 16u : 2u),
                        dim3(64 * kLoraInWaves), 0, s, a);
     const int nb = EACH ? 1 : (int)(((long)blocks * f.v[4] + 511) / 512);
     const dim3 g((unsigned)((blocks + nb - 1) / nb), (unsigned)f.v[4], EACH ? 16u : 1u), b(64 * kLoraOutWaves);
