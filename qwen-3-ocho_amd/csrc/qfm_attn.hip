@@ -245,7 +245,7 @@ struct Tile {
 };
 
 template <int FMT, int D, int RB, int DT>
-__global__ void __launch_bounds__(64 * kAttnWaves, RB * D <= 256 ? 2 : 1)
+__global__ void __launch_bounds__(64 * kAttnWaves, RB * D <= 256 ? 2 : 1)   // 256 registers: beyond, the compiler copies results in and out of accumulation registers
 k_tree_attn(KvView c, AttnArgs a) {
     constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), ROWS = 16 * RB, LD = D + 4;
     __shared__ float s_o[kAttnWaves][ROWS * LD];
@@ -476,7 +476,7 @@ k_tree_attn(KvView c, AttnArgs a) {
     }
 }
 
-// The same for many rows (more than kFewRows of a key/value head): eight waves,
+// The same for many rows of a key/value head: eight waves,
 // 8 / WT of them with 16 RB rows each, in WT groups that take the tiles in turn.
 // A tile is widened to fp16 once, by all waves, and laid into LDS in the order
 // of the MFMA operands (16-byte reads and writes, no two lanes on a bank); each
@@ -861,39 +861,60 @@ k_tree_join_few(AttnArgs a, int heads) {
     store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-// How a call is laid out: 16 RB rows a wave; few rows (wt 0) as k_tree_attn, more
-// as k_tree_wide with wt groups of waves; and the splits of a sequence's keys.
+// How a call is laid out: 16 rb rows a wave, in k_tree_attn (wt 0) or k_tree_wide
+// (wt groups of waves), and the splits of a sequence's keys.
 struct AttnPlan { int rb, wt, block, splits; };      // block: rows a workgroup
-constexpr int kFewRows = 64;
-constexpr int few_blocks(int D, int rows, bool f32) {
-    const int most = D == 64 ? 4 : D == 128 ? (f32 ? 2 : 4) : f32 ? 1 : 2, want = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    return want < most ? want : most;
-}
-// wide: the rows a wave holds within 256 registers
-constexpr int wide_blocks(int D, bool f32) { return D == 64 ? 2 : D == 128 && !f32 ? 2 : 1; }
+// what a wave holds within 256 registers
+constexpr int few_blocks(int D, bool f32) { return D == 256 && f32 ? 1 : 2; }
+constexpr int wide_blocks(int D, bool f32) { return D == 64 || (D == 128 && !f32) ? 2 : 1; }
 // workgroups that a CU holds at once
-constexpr int few_resident(int D, int rb) { return rb == 1 && D <= 128 ? 2 : rb == 2 && D == 64 ? 2 : 1; }
+constexpr int few_resident(int D, int rb) { return rb == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2; }
+
+// Microseconds that a layout takes, as fitted to 70 shapes (contexts 1 to 131071,
+// 1 to 64 nodes, every head layout and type) in up to 40 layouts each: rounds of
+// resident workgroups, each a prologue and its tiles; a step is as long as its
+// loads' latency or as what the CU's workgroups compute together; a join and its
+// partial results. What it picks takes 2% more than the best layout on average;
+// one round of resident workgroups with the widest rows took 19% more, and
+// without k_tree_wide it would be 3.5% (61-node trees of five users 81 us, 73).
+static float attn_cost(const AttnPlan &p, int D, bool f32, long groups, int rows, long tiles) {
+    const float d = D / 128.0f, each = p.wt ? p.wt : kAttnWaves;
+    const int resident = p.wt ? 1 : few_resident(D, p.rb);
+    const long all = groups * p.splits, rounds = (all + 256 * resident - 1) / (256 * resident);
+    const float occ = (float)min((long)resident, (all + 255) / 256);
+    const float steps = (float)(long)((tiles + p.splits * (long)each - 1) / (p.splits * (long)each));
+    const float busy = occ * d * (p.rb == 1 ? 0.49f : 0.62f) * (f32 ? 1.2f : 1.0f);
+    const float step = p.wt ? 0.09f + 0.58f * d * p.rb : max(0.42f + 0.69f * d, busy);
+    float us = 5.1f + rounds * ((p.wt ? 2.8f : 0.56f) + 0.45f * d * p.rb + steps * step);
+    if (p.splits > 1) us += 3.2f + (float)all * min(p.block, rows) * D * 8 / 3.2e6f;
+    return us;
+}
 
 static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, bool f32) {
+    static const int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxSplits};
     const int rows = max_nodes * (q_heads / kv_heads);
-    AttnPlan p{};
-    int resident;
-    if (rows <= kFewRows) {
-        p.rb = few_blocks(D, rows, f32);
-        p.block = 16 * p.rb;
-        resident = few_resident(D, p.rb);
-    } else {
-        p.rb = wide_blocks(D, f32);
-        p.wt = rows <= 4 * 16 * p.rb ? 2 : 1;
-        p.block = 16 * p.rb * (kWideWaves / p.wt);
-        resident = 1;
+    const long tiles = ((long)max_ctx + max_nodes + 31) / 32;
+    AttnPlan best{};
+    float least = 0.0f;
+    for (int form = 0; form < 4; form++) {                  // rb 1, rb 2, wide in two groups, wide in one
+        AttnPlan p{};
+        p.wt = form < 2 ? 0 : 4 - form;
+        p.rb = form < 2 ? form + 1 : wide_blocks(D, f32);
+        if (form == 1 && few_blocks(D, f32) < 2) continue;
+        if (form && rows <= 16) break;
+        p.block = 16 * p.rb * (p.wt ? kWideWaves / p.wt : 1);
+        const long groups = (long)n_seq * kv_heads * ((rows + p.block - 1) / p.block);
+        for (int n : kSplits) {
+            if (n > 1 && n > tiles) break;
+            p.splits = n;
+            const float us = attn_cost(p, D, f32, groups, rows, tiles);
+            if (!best.rb || us < least) {
+                best = p;
+                least = us;
+            }
+        }
     }
-    // one round of resident workgroups over the 256 CUs, each with a tile or more
-    // for every wave (or group of waves)
-    const long groups = (long)n_seq * kv_heads * ((rows + p.block - 1) / p.block);
-    const long tiles = ((long)max_ctx + max_nodes + 31) / 32, each = p.wt ? 2 * p.wt : kAttnWaves;
-    p.splits = (int)max(1l, min(min((long)kMaxSplits, 256 * resident / groups), (tiles + each - 1) / each));
-    return p;
+    return best;
 }
 
 static int attn_shape(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
@@ -911,18 +932,12 @@ static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
 template <int FMT, int D, int DT>
 static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, dim3 g, hipStream_t s) {
     constexpr bool F32 = DT == QFM_DT_F32;
-    constexpr int RB = wide_blocks(D, F32), MOST = few_blocks(D, kFewRows, F32);
+    constexpr int RB = wide_blocks(D, F32);
     const dim3 b(64 * kAttnWaves), bw(64 * kWideWaves);
     if (p.wt == 1) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 1>), g, bw, 0, s, v, a);
     else if (p.wt == 2) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 2>), g, bw, 0, s, v, a);
-    else if (p.wt == 4) {
-        if constexpr (D <= 128) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 4>), g, bw, 0, s, v, a);
-    } else if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, DT>), g, b, 0, s, v, a);
-    else if (p.rb == 2) {
-        if constexpr (MOST >= 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, DT>), g, b, 0, s, v, a);
-    } else {
-        if constexpr (MOST >= 4) hipLaunchKernelGGL((k_tree_attn<FMT, D, 4, DT>), g, b, 0, s, v, a);
-    }
+    else if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, DT>), g, b, 0, s, v, a);
+    else if constexpr (few_blocks(D, F32) == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, DT>), g, b, 0, s, v, a);
 }
 template <int D, int DT>
 static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, int fmt, int n_seq, hipStream_t s) {
