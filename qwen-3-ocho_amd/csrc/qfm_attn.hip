@@ -237,17 +237,21 @@ __device__ __forceinline__ uint64_t node_mask(const AttnArgs &a, int first, int 
     return a.tree ? a.tree[first + node] : node == 63 ? ~0ull : (2ull << node) - 1;
 }
 
-// a 32-token tile of keys and values, as the lanes hold it
+// a 32-token tile of keys or values, as the lanes hold it; scale (with the keys):
+// of key lane (lane < 32) or of value lane - 32
 template <int NC>
 struct Tile {
-    u32x4_t k[2][NC], v[2][NC];
-    float4 ks[2], vs[2];
+    u32x4_t x[2][NC];
+    float scale;
 };
 
 template <int FMT, int D, int RB, int DT>
 __global__ void __launch_bounds__(64 * kAttnWaves, RB * D <= 256 ? 2 : 1)   // 256 registers: beyond, the compiler copies results in and out of accumulation registers
 k_tree_attn(KvView c, AttnArgs a) {
     constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), ROWS = 16 * RB, LD = D + 4;
+    // two tiles in registers, where there are so many
+    constexpr bool DEEP = RB * D <= 128;
+    __shared__ __attribute__((aligned(16))) float s_sc[kAttnWaves][64];
     __shared__ float s_o[kAttnWaves][ROWS * LD];
     __shared__ float s_m[kAttnWaves][ROWS], s_l[kAttnWaves][ROWS];
     __shared__ int s_ve[kAttnWaves];
@@ -272,25 +276,27 @@ k_tree_attn(KvView c, AttnArgs a) {
         y = p + 16 < len && (unsigned)y < (unsigned)c.n_pages ? y : -1;
         return make_int2(x, y);
     };
-    Tile<NC> w;
-    auto load_k = [&](int tt, int2 pg) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const size_t at = c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
-#pragma unroll
-            for (int k = 0; k < NC; k++)
-                w.k[i][k] = *reinterpret_cast<const u32x4_t *>(c.k + at * D + l16 * D + 64 * k + 16 * g);
-            w.ks[i] = *reinterpret_cast<const float4 *>(c.ks + at + 4 * g);
-        }
+    auto half_at = [&](int tt, int i, int2 pg) {
+        return c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
     };
-    auto load_v = [&](int tt, int2 pg) {
+    auto load_k = [&](Tile<NC> &w, int tt, int2 pg) {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const size_t at = c.token0(max(i ? pg.y : pg.x, 0), h) + ((32 * tt + 16 * i) & (c.page() - 1));
+            const size_t at = half_at(tt, i, pg);
 #pragma unroll
             for (int k = 0; k < NC; k++)
-                w.v[i][k] = *reinterpret_cast<const u32x4_t *>(c.v + at * D + 4 * g * D + (64 * k + 4 * l16) * 4);
-            w.vs[i] = *reinterpret_cast<const float4 *>(c.vs + at + 4 * g);
+                w.x[i][k] = *reinterpret_cast<const u32x4_t *>(c.k + at * D + l16 * D + 64 * k + 16 * g);
+        }
+        const size_t at = g & 1 ? half_at(tt, 1, pg) : half_at(tt, 0, pg);
+        w.scale = (lane < 32 ? c.ks : c.vs)[at + l16];
+    };
+    auto load_v = [&](Tile<NC> &w, int tt, int2 pg) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t at = half_at(tt, i, pg);
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                w.x[i][k] = *reinterpret_cast<const u32x4_t *>(c.v + at * D + 4 * g * D + (64 * k + 4 * l16) * 4);
         }
     };
     // Q: the waves share the row blocks out and leave their fragments in LDS; up to
@@ -306,10 +312,11 @@ k_tree_attn(KvView c, AttnArgs a) {
         if ((rb & (kAttnWaves - 1)) == wave) q[rb].load(a, sr.x, h, r, node, g);
         R.see[rb] = node_mask(a, sr.x, node);
     }
+    Tile<NC> kt[DEEP ? 2 : 1], vt[DEEP ? 2 : 1];
     int2 pg = pages(t);
     if (t < t1) {
-        load_k(t, pg);
-        load_v(t, pg);
+        load_k(kt[0], t, pg);
+        load_v(vt[0], t, pg);
     }
     int2 pn = pages(t + kAttnWaves);
 #pragma unroll
@@ -344,11 +351,15 @@ k_tree_attn(KvView c, AttnArgs a) {
     };
 
     R.clear();
-    // A tile's keys are used up before its values: the next keys are requested
-    // ahead of the softmax, the next values behind the second product, into the
-    // registers that have just become free.
-    while (t < t1) {
+    // One tile. DEEP: its successor is requested first, into registers of its
+    // own; else the keys ahead of the softmax and the
+    // values behind the second product, into the registers that have just become
+    // free.
+    auto step = [&](Tile<NC> &kn, Tile<NC> &kx, Tile<NC> &vn, Tile<NC> &vx) {
         const bool more = t + kAttnWaves < t1;
+        if (DEEP && more) load_k(kx, t + kAttnWaves, pn);
+        if (DEEP && more) load_v(vx, t + kAttnWaves, pn);
+        s_sc[wave][lane] = kn.scale;
         int again = 0;                     // what the compiler cannot see through: Q is not to be kept in registers
         asm volatile("" : "+v"(again));
         f32x4_t s[RB][2];
@@ -359,7 +370,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < NC; k++) {
                 f16x8_t ka, kb;
-                codes16<FMT>(w.k[i][k], ka, kb);
+                codes16<FMT>(kn.x[i][k], ka, kb);
 #pragma unroll
                 for (int n = 0; n < QP; n++) {
 #pragma unroll
@@ -368,16 +379,21 @@ k_tree_attn(KvView c, AttnArgs a) {
                     for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(kb, q_of(rb, k, 1, n, again), s[rb][i]);
                 }
             }
+        wave_lds_fence();
+        float vs[2][4];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const float ks[4] = {w.ks[i].x, w.ks[i].y, w.ks[i].z, w.ks[i].w};
+            const f32x4_t x = *reinterpret_cast<const f32x4_t *>(&s_sc[wave][16 * i + 4 * g]);
+            const f32x4_t y = *reinterpret_cast<const f32x4_t *>(&s_sc[wave][32 + 16 * i + 4 * g]);
 #pragma unroll
-            for (int rb = 0; rb < RB; rb++)
+            for (int e = 0; e < 4; e++) {
+                vs[i][e] = y[e];
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[e];
+                for (int rb = 0; rb < RB; rb++) s[rb][i][e] *= x[e];
+            }
         }
-        if (more) load_k(t + kAttnWaves, pn);
-        float vs[2][4] = {{w.vs[0].x, w.vs[0].y, w.vs[0].z, w.vs[0].w}, {w.vs[1].x, w.vs[1].y, w.vs[1].z, w.vs[1].w}};
+        wave_lds_fence();
+        if (!DEEP && more) load_k(kx, t + kAttnWaves, pn);
         if (32 * t + 32 > ctx || (pg.x | pg.y) < 0) {
             const int j0[2] = {32 * t + 4 * g, 32 * t + 16 + 4 * g};
             const int n4[2] = {pg.x < 0 ? 0 : min(max(len - j0[0], 0), 4), pg.y < 0 ? 0 : min(max(len - j0[1], 0), 4)};
@@ -389,7 +405,7 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                     for (int k = 0; k < NC; k++)
 #pragma unroll
-                        for (int q = 0; q < 4; q++) w.v[i][k][q] &= token_bytes(n4[i]);
+                        for (int q = 0; q < 4; q++) vn.x[i][k][q] &= token_bytes(n4[i]);
             }
         }
         f16x8_t pf[RB][PP];
@@ -398,8 +414,8 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
         for (int k = 0; k < NC; k++) {
             f16x8_t a0, b0, a1, b1;
-            codes16<FMT>(w.v[0][k], a0, b0);
-            codes16<FMT>(w.v[1][k], a1, b1);
+            codes16<FMT>(vn.x[0][k], a0, b0);
+            codes16<FMT>(vn.x[1][k], a1, b1);
             const f16x8_t vf[4] = {__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 8, 9, 10, 11),
                                    __builtin_shufflevector(a0, a1, 4, 5, 6, 7, 12, 13, 14, 15),
                                    __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 8, 9, 10, 11),
@@ -411,10 +427,17 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
                     for (int n = 0; n < PP; n++) R.o[rb][k][q] = mfma_f16(vf[q], pf[rb][n], R.o[rb][k][q]);
         }
+        if (!DEEP && more) load_v(vx, t + kAttnWaves, pn);
         t += kAttnWaves;
-        if (more) load_v(t, pn);
         pg = pn;
         pn = pages(t + kAttnWaves);
+    };
+    while (t < t1) {
+        step(kt[0], kt[DEEP], vt[0], vt[DEEP]);
+        if constexpr (DEEP) {
+            if (t >= t1) break;
+            step(kt[1], kt[0], vt[1], vt[0]);
+        }
     }
 
     // join the waves
