@@ -24,6 +24,7 @@
 #include "qfm_kv.h"
 #include "qfm_mfma.h"
 #include "qfm_internal.h"
+#include <algorithm>
 
 namespace qfm {
 
@@ -499,27 +500,24 @@ k_tree_attn(KvView c, AttnArgs a) {
     }
 }
 
-// The same for many rows of a key/value head: eight waves,
-// 8 / WT of them with 16 RB rows each, in WT groups that take the tiles in turn.
-// A tile is widened to fp16 once, by all waves, and laid into LDS in the order
+// The same for many rows of a key/value head: eight waves of 16 RB rows each,
+// which take every tile together. It is widened to fp16 once, by all waves, and laid into LDS in the order
 // of the MFMA operands (16-byte reads and writes, no two lanes on a bank); each
 // step's tiles are requested a step ahead of being widened and widened a step
 // ahead of their use, one barrier a step.
 constexpr int kWideWaves = 8;
 
-template <int FMT, int D, int RB, int DT, int WT>
+template <int FMT, int D, int RB, int DT>
 __global__ void __launch_bounds__(64 * kWideWaves)
 k_tree_wide(KvView c, AttnArgs a) {
-    constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), WR = kWideWaves / WT, ROWS = 16 * RB * WR;
+    constexpr int NC = D / 64, QP = q_parts(DT), PP = p_parts(DT), ROWS = 16 * RB * kWideWaves;
     constexpr int NF = 8 * NC;                              // fragments a tile: 4 NC of K, then 4 NC of V
-    constexpr int UNITS = WT * 4 * NC, UN = (UNITS + kWideWaves - 1) / kWideWaves, LJ = 68;
-    constexpr int TILES = 2 * WT * NF * 64 * 16, JOIN = kWideWaves * 16 * (WT > 1 ? RB : 1) * LJ * 4;
+    constexpr int UNITS = 4 * NC, UN = (UNITS + kWideWaves - 1) / kWideWaves, LJ = 68;
+    constexpr int TILES = 2 * NF * 64 * 16, JOIN = kWideWaves * 16 * LJ * 4;
     __shared__ __attribute__((aligned(16))) uint8_t s_buf[TILES > JOIN ? TILES : JOIN];
-    __shared__ float s_sc[2][WT][64];                       // 32 key scales, 32 value scales
-    __shared__ float s_m[kWideWaves][16 * RB], s_l[kWideWaves][16 * RB];
-    __shared__ int s_ve[kWideWaves];
+    __shared__ float s_sc[2][64];                           // 32 key scales, 32 value scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int g = lane >> 4, l16 = lane & 15, wr = wave % WR, wt = wave / WR;
+    const int g = lane >> 4, l16 = lane & 15;
     const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
     const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
     const int rows = sr.y * a.G, row0 = blk * ROWS;
@@ -527,9 +525,9 @@ k_tree_wide(KvView c, AttnArgs a) {
     const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
     const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
     const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
-    const int t0 = (int)blockIdx.x * per, t1 = min(nt, t0 + per), steps = (t1 - t0 + WT - 1) / WT;
+    const int t0 = (int)blockIdx.x * per, t1 = min(nt, t0 + per);
     const int lim = min(len, 32 * t1);                      // tokens from here on are no keys of this workgroup
-    const bool live = row0 + 16 * RB * wr < rows;           // this wave has rows
+    const bool live = row0 + 16 * RB * wave < rows;           // this wave has rows
 
     const int *table = c.table + (size_t)seq * c.max_pages;
     auto pages = [&](int tt) {
@@ -545,35 +543,28 @@ k_tree_wide(KvView c, AttnArgs a) {
     };
     u32x4_t raw[UN];
     float raw_sc;
-    auto request = [&](int step, const int2 (&pg)[WT]) {
+    auto request = [&](int tt, int2 pg) {
 #pragma unroll
         for (int n = 0; n < UN; n++) {
-            const int u = wave + kWideWaves * n, w = u / (4 * NC), r = u % (4 * NC), i = (r % (2 * NC)) / NC, k = r % NC;
-            if (u >= UNITS) break;
-            int2 p = pg[0];
-#pragma unroll
-            for (int v = 1; v < WT; v++) p = w == v ? pg[v] : p;
-            const size_t at = half_at(t0 + step * WT + w, i, p);
+            const int r = wave + kWideWaves * n, i = (r % (2 * NC)) / NC, k = r % NC;
+            if (r >= UNITS) break;
+            const size_t at = half_at(tt, i, pg);
             const uint8_t *src = r < 2 * NC ? c.k + at * D + l16 * D + 64 * k + 16 * g
                                             : c.v + at * D + 4 * g * D + (64 * k + 4 * l16) * 4;
             raw[n] = *reinterpret_cast<const u32x4_t *>(src);
         }
-        if (wave < WT) {
-            int2 p = pg[0];
-#pragma unroll
-            for (int v = 1; v < WT; v++) p = wave == v ? pg[v] : p;
-            const int tt = t0 + step * WT + wave, i = (lane >> 4) & 1;
-            const size_t at = half_at(tt, i, p) + l16;
+        if (wave == 0) {
+            const size_t at = half_at(tt, (lane >> 4) & 1, pg) + l16;
             raw_sc = (lane < 32 ? c.ks : c.vs)[at];
         }
     };
-    auto widen = [&](int step, const int2 (&pg)[WT]) {
-        uint8_t *buf = s_buf + (step & 1) * (TILES / 2);
+    auto widen = [&](int tt, int2 pg) {
+        uint8_t *buf = s_buf + (tt & 1) * (TILES / 2);
 #pragma unroll
         for (int n = 0; n < UN; n++) {
-            const int u = wave + kWideWaves * n, w = u / (4 * NC), r = u % (4 * NC), i = (r % (2 * NC)) / NC, k = r % NC;
-            if (u >= UNITS) break;
-            uint8_t *dst = buf + (size_t)w * (NF * 1024) + lane * 16;
+            const int r = wave + kWideWaves * n, i = (r % (2 * NC)) / NC, k = r % NC;
+            if (r >= UNITS) break;
+            uint8_t *dst = buf + lane * 16;
             f16x8_t x, y;
             if (r < 2 * NC) {
                 codes16<FMT>(raw[n], x, y);
@@ -581,11 +572,8 @@ k_tree_wide(KvView c, AttnArgs a) {
                 *reinterpret_cast<f16x8_t *>(dst + ((i * NC + k) * 2 + 1) * 1024) = y;
             } else {
                 if constexpr (FMT == QFM_KV_E4M3) {
-                    int2 p = pg[0];
-#pragma unroll
-                    for (int v = 1; v < WT; v++) p = w == v ? pg[v] : p;
-                    const int j0 = 32 * (t0 + step * WT + w) + 16 * i + 4 * g;
-                    const uint32_t keep = token_bytes((i ? p.y : p.x) < 0 ? 0 : min(max(lim - j0, 0), 4));
+                    const int j0 = 32 * tt + 16 * i + 4 * g;
+                    const uint32_t keep = token_bytes((i ? pg.y : pg.x) < 0 ? 0 : min(max(lim - j0, 0), 4));
 #pragma unroll
                     for (int q = 0; q < 4; q++) raw[n][q] &= keep;
                 }
@@ -598,40 +586,30 @@ k_tree_wide(KvView c, AttnArgs a) {
                 *reinterpret_cast<u32x2_t *>(dst + 3072) = u32x2_t{q[2], q[3]};
             }
         }
-        if (wave < WT) s_sc[step & 1][wave][lane] = raw_sc;
+        if (wave == 0) s_sc[tt & 1][lane] = raw_sc;
     };
     Rows<RB, NC, PP> R;
     QRow<NC, DT> q[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
-        const int r = min(row0 + 16 * (RB * wr + rb) + l16, rows - 1), node = r / a.G;
+        const int r = min(row0 + 16 * (RB * wave + rb) + l16, rows - 1), node = r / a.G;
         q[rb].load(a, sr.x, h, r, node, g);
         R.see[rb] = node_mask(a, sr.x, node);
     }
-    int2 pc[WT], pn[WT], pf2[WT];                           // pages of this step's tiles and of the next two
-#pragma unroll
-    for (int w = 0; w < WT; w++) {
-        pc[w] = pages(t0 + w);
-        pn[w] = pages(t0 + WT + w);
-        pf2[w] = pages(t0 + 2 * WT + w);
-    }
-    if (steps > 0) request(0, pc);
+    int2 pc = pages(t0), pn = pages(t0 + 1), pf2 = pages(t0 + 2);   // of this tile and the next two
+    if (t0 < t1) request(t0, pc);
     f16x8_t qf[RB][NC][2][QP];
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) R.qs[rb] = q[rb].widen(a.scale, qf[rb]);
     R.clear();
-    if (steps > 0) widen(0, pc);
-    if (steps > 1) request(1, pn);
+    if (t0 < t1) widen(t0, pc);
+    if (t0 + 1 < t1) request(t0 + 1, pn);
     __syncthreads();
-    for (int st = 0; st < steps; st++) {
-        if (st + 1 < steps) widen(st + 1, pn);
-        if (st + 2 < steps) request(st + 2, pf2);
+    for (int t = t0; t < t1; t++) {
+        if (t + 1 < t1) widen(t + 1, pn);
+        if (t + 2 < t1) request(t + 2, pf2);
         if (live) {
-            const uint8_t *buf = s_buf + (st & 1) * (TILES / 2) + wt * (NF * 1024) + lane * 16;
-            const int t = t0 + st * WT + wt;
-            int2 pg = pc[0];
-#pragma unroll
-            for (int v = 1; v < WT; v++) pg = wt == v ? pc[v] : pg;
+            const uint8_t *buf = s_buf + (t & 1) * (TILES / 2) + lane * 16;
             f32x4_t s[RB][2];
 #pragma unroll
             for (int rb = 0; rb < RB; rb++) s[rb][0] = s[rb][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -648,7 +626,7 @@ k_tree_wide(KvView c, AttnArgs a) {
                             for (int rb = 0; rb < RB; rb++) s[rb][i] = mfma_f16(kf, qf[rb][k][j][n], s[rb][i]);
                     }
             float vs[2][4];
-            const float *sc = s_sc[st & 1][wt];
+            const float *sc = s_sc[t & 1];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 const float4 x = *reinterpret_cast<const float4 *>(sc + 16 * i + 4 * g);
@@ -660,9 +638,9 @@ k_tree_wide(KvView c, AttnArgs a) {
 #pragma unroll
                     for (int e = 0; e < 4; e++) s[rb][i][e] *= ks[e];
             }
-            if (32 * t + 32 > min(ctx, lim) || (pg.x | pg.y) < 0) {
+            if (32 * t + 32 > min(ctx, lim) || (pc.x | pc.y) < 0) {
                 const int j0[2] = {32 * t + 4 * g, 32 * t + 16 + 4 * g};
-                const int n4[2] = {pg.x < 0 ? 0 : min(max(lim - j0[0], 0), 4), pg.y < 0 ? 0 : min(max(lim - j0[1], 0), 4)};
+                const int n4[2] = {pc.x < 0 ? 0 : min(max(lim - j0[0], 0), 4), pc.y < 0 ? 0 : min(max(lim - j0[1], 0), 4)};
                 const int node0[2] = {j0[0] - ctx, j0[1] - ctx};
                 R.hide(s, vs, n4, node0);
             }
@@ -679,12 +657,9 @@ k_tree_wide(KvView c, AttnArgs a) {
                         for (int rb = 0; rb < RB; rb++) R.o[rb][k][q] = mfma_f16(vf, pf[rb][n], R.o[rb][k][q]);
                 }
         }
-#pragma unroll
-        for (int w = 0; w < WT; w++) {
-            pc[w] = pn[w];
-            pn[w] = pf2[w];
-            pf2[w] = pages(t0 + (st + 3) * WT + w);
-        }
+        pc = pn;
+        pn = pf2;
+        pf2 = pages(t + 3);
         __syncthreads();
     }
 
@@ -700,85 +675,32 @@ k_tree_wide(KvView c, AttnArgs a) {
         if (a.splits == 1) store4<DT>(a.out, p.t * a.ors + p.head * a.ohs + d, x);
         else *reinterpret_cast<float4 *>(a.po + p.at * D + d) = x;
     };
-    float *s_j = reinterpret_cast<float *>(s_buf);          // WT 1: [waves][16][LJ], else [waves][16 RB][LJ]
+    float *s_j = reinterpret_cast<float *>(s_buf) + wave * (16 * LJ);
+    if (!live) return;
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) R.l[rb] = sum_over_g(R.l[rb]);
-    if constexpr (WT == 1) {
-        if (!live) return;
-        s_j += wave * (16 * LJ);
-        const float back = exp2i(R.ve - 6);
+    const float back = exp2i(R.ve - 6);
 #pragma unroll
-        for (int rb = 0; rb < RB; rb++) {
-            const int r0 = row0 + 16 * (RB * wr + rb);
-            const float inv = R.l[rb] == 0.0f ? 0.0f : back / R.l[rb];
-            if (a.splits > 1 && g == 0 && r0 + l16 < rows) a.pml[place(r0 + l16).at] = make_float2(R.m[rb], R.l[rb]);
-            Place p[4];
+    for (int rb = 0; rb < RB; rb++) {
+        const int r0 = row0 + 16 * (RB * wave + rb);
+        const float inv = R.l[rb] == 0.0f ? 0.0f : back / R.l[rb];
+        if (a.splits > 1 && g == 0 && r0 + l16 < rows) a.pml[place(r0 + l16).at] = make_float2(R.m[rb], R.l[rb]);
+        Place p[4];
 #pragma unroll
-            for (int n = 0; n < 4; n++) p[n] = place(min(r0 + 4 * n + g, rows - 1));
-#pragma unroll
-            for (int k = 0; k < NC; k++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(&s_j[l16 * LJ + 16 * g + 4 * i]) =
-                        make_float4(R.o[rb][k][0][i] * inv, R.o[rb][k][1][i] * inv, R.o[rb][k][2][i] * inv, R.o[rb][k][3][i] * inv);
-                wave_lds_fence();
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(&s_j[(4 * n + g) * LJ + 4 * l16]);
-                    if (r0 + 4 * n + g < rows) put(p[n], 64 * k + 4 * l16, x);
-                }
-                wave_lds_fence();
-            }
-        }
-    } else {
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++)
-            if (g == 0) {
-                s_m[wave][16 * rb + l16] = R.m[rb];
-                s_l[wave][16 * rb + l16] = R.l[rb];
-            }
-        if (lane == 0) s_ve[wave] = R.ve;
-        __syncthreads();
-        int vn = s_ve[0];
-#pragma unroll
-        for (int w = 1; w < kWideWaves; w++) vn = max(vn, s_ve[w]);
-        float f[RB];
-#pragma unroll
-        for (int rb = 0; rb < RB; rb++) {
-            float mn = kNoMax;
-#pragma unroll
-            for (int w = 0; w < WT; w++) mn = fmaxf(mn, s_m[w * WR + wr][16 * rb + l16]);
-            f[rb] = __builtin_amdgcn_exp2f(R.m[rb] - mn) * pow2_ratio(R.ve - vn);
-        }
-        const float back = exp2i(vn - 6);
+        for (int n = 0; n < 4; n++) p[n] = place(min(r0 + 4 * n + g, rows - 1));
 #pragma unroll
         for (int k = 0; k < NC; k++) {
 #pragma unroll
-            for (int rb = 0; rb < RB; rb++)
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4 *>(&s_j[l16 * LJ + 16 * g + 4 * i]) =
+                    make_float4(R.o[rb][k][0][i] * inv, R.o[rb][k][1][i] * inv, R.o[rb][k][2][i] * inv, R.o[rb][k][3][i] * inv);
+            wave_lds_fence();
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    *reinterpret_cast<float4 *>(&s_j[(wave * 16 * RB + 16 * rb + l16) * LJ + 16 * g + 4 * i]) =
-                        make_float4(R.o[rb][k][0][i] * f[rb], R.o[rb][k][1][i] * f[rb], R.o[rb][k][2][i] * f[rb], R.o[rb][k][3][i] * f[rb]);
-            __syncthreads();
-            for (int e = threadIdx.x; e < ROWS * 16; e += 64 * kWideWaves) {
-                const int r = e >> 4, d = (e & 15) * 4, rw = r / (16 * RB), rr = r % (16 * RB);
-                if (row0 + r >= rows) break;
-                float mn = kNoMax, sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WT; w++) mn = fmaxf(mn, s_m[w * WR + rw][rr]);
-                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int w = 0; w < WT; w++) {
-                    const float4 y = *reinterpret_cast<const float4 *>(&s_j[((w * WR + rw) * 16 * RB + rr) * LJ + d]);
-                    x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-                    sum += s_l[w * WR + rw][rr] * __builtin_amdgcn_exp2f(s_m[w * WR + rw][rr] - mn);
-                }
-                const float inv = sum == 0.0f ? 0.0f : back / sum;
-                const Place p = place(row0 + r);
-                put(p, 64 * k + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
-                if (a.splits > 1 && k + d == 0) a.pml[p.at] = make_float2(mn, sum);
+            for (int n = 0; n < 4; n++) {
+                const float4 x = *reinterpret_cast<const float4 *>(&s_j[(4 * n + g) * LJ + 4 * l16]);
+                if (r0 + 4 * n + g < rows) put(p[n], 64 * k + 4 * l16, x);
             }
-            __syncthreads();
+            wave_lds_fence();
         }
     }
 }
@@ -884,53 +806,59 @@ k_tree_join_few(AttnArgs a, int heads) {
     store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-// How a call is laid out: 16 rb rows a wave, in k_tree_attn (wt 0) or k_tree_wide
-// (wt groups of waves), and the splits of a sequence's keys.
-struct AttnPlan { int rb, wt, block, splits; };      // block: rows a workgroup
+// How a call is laid out: 16 rb rows a wave, in k_tree_attn or k_tree_wide, and
+// the splits of a sequence's keys.
+struct AttnPlan { int rb, block, splits; bool wide; };      // block: rows a workgroup
 // what a wave holds within 256 registers
 constexpr int few_blocks(int D, bool f32) { return D == 256 && f32 ? 1 : 2; }
 constexpr int wide_blocks(int D, bool f32) { return D == 64 || (D == 128 && !f32) ? 2 : 1; }
-// workgroups that a CU holds at once
-constexpr int few_resident(int D, int rb) { return rb == 1 ? (D == 64 ? 4 : D == 128 ? 3 : 2) : D == 256 ? 1 : 2; }
+// workgroups that a CU holds at once, by their registers
+constexpr int few_resident(int D, int rb) { return rb == 1 ? (D == 64 ? 3 : 2) : D == 256 ? 1 : 2; }
 
-// Microseconds that a layout takes, as fitted to 70 shapes (contexts 1 to 131071,
+// Microseconds that a layout takes, as fitted to 130 shapes (contexts 1 to 131071,
 // 1 to 64 nodes, every head layout and type) in up to 40 layouts each: rounds of
-// resident workgroups, each a prologue and its tiles; a step is as long as its
-// loads' latency or as what the CU's workgroups compute together; a join and its
-// partial results. What it picks takes 2% more than the best layout on average;
-// one round of resident workgroups with the widest rows took 19% more, and
-// without k_tree_wide it would be 3.5% (61-node trees of five users 81 us, 73).
-static float attn_cost(const AttnPlan &p, int D, bool f32, long groups, int rows, long tiles) {
-    const float d = D / 128.0f, each = p.wt ? p.wt : kAttnWaves;
-    const int resident = p.wt ? 1 : few_resident(D, p.rb);
-    const long all = groups * p.splits, rounds = (all + 256 * resident - 1) / (256 * resident);
-    const float occ = (float)min((long)resident, (all + 255) / 256);
+// resident workgroups (fractions of one for the most part: sequences differ in
+// length), each a prologue and its tiles; a step is as long as its loads' latency
+// or as what the CU's workgroups compute together; a join and its partial results.
+// What it picks takes 1.3% more than the best layout on average; one round of
+// resident workgroups with the widest rows took 22% more. Each form is there for
+// what the others lose without it: 16 rows a wave 17%, 32 rows 4%, k_tree_wide 3%
+// (61-node trees of five users: 84 us, 75 with it).
+static float attn_cost(const AttnPlan &p, int D, int dtype, long groups, int rows, long tiles) {
+    const float d = D / 128.0f, each = p.wide ? 1 : kAttnWaves;
+    const bool f32 = dtype == QFM_DT_F32, f16 = dtype == QFM_DT_F16;
+    const int resident = p.wide ? 1 : few_resident(D, p.rb);
+    const long all = groups * p.splits, whole = (all + 256 * resident - 1) / (256 * resident);
+    const float rounds = 0.24f * whole + 0.76f * std::max(1.0f, all / (256.0f * resident));
+    const float occ = (float)std::min<long>(resident, (all + 255) / 256);
     const float steps = (float)(long)((tiles + p.splits * (long)each - 1) / (p.splits * (long)each));
-    const float busy = occ * d * (p.rb == 1 ? 0.49f : 0.62f) * (f32 ? 1.2f : 1.0f);
-    const float step = p.wt ? 0.09f + 0.58f * d * p.rb : max(0.42f + 0.69f * d, busy);
-    float us = 5.1f + rounds * ((p.wt ? 2.8f : 0.56f) + 0.45f * d * p.rb + steps * step);
-    if (p.splits > 1) us += 3.2f + (float)all * min(p.block, rows) * D * 8 / 3.2e6f;
+    const float busy = occ * d * (p.rb == 1 ? 0.66f : 0.83f) * (f32 ? 0.89f : f16 ? 0.69f : 1.0f);
+    const float wait = (0.37f + 0.55f * d) * (p.rb * D > 128 ? 1.14f : 1.0f);
+    const float step = p.wide ? 0.15f + 0.43f * d * p.rb * (f32 ? 1.9f : f16 ? 1.19f : 1.0f) : std::max(wait, busy);
+    float us = 3.9f + rounds * ((p.wide ? 2.2f : 1.1f) + 1.1f * d * p.rb + steps * step);
+    if (p.splits > 1) us += 3.1f + (p.splits > kFewSplits ? 1.4f : 0.0f) + (float)all * std::min(p.block, rows) * D * 8 / 5.4e6f;
     return us;
 }
 
-static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, bool f32) {
+static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, int dtype) {
     static const int kSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, kMaxSplits};
     const int rows = max_nodes * (q_heads / kv_heads);
     const long tiles = ((long)max_ctx + max_nodes + 31) / 32;
+    const bool f32 = dtype == QFM_DT_F32;
     AttnPlan best{};
     float least = 0.0f;
-    for (int form = 0; form < 4; form++) {                  // rb 1, rb 2, wide in two groups, wide in one
+    for (int form = 0; form < 3; form++) {                  // rb 1, rb 2, wide
         AttnPlan p{};
-        p.wt = form < 2 ? 0 : 4 - form;
-        p.rb = form < 2 ? form + 1 : wide_blocks(D, f32);
+        p.wide = form == 2;
+        p.rb = p.wide ? wide_blocks(D, f32) : form + 1;
         if (form == 1 && few_blocks(D, f32) < 2) continue;
         if (form && rows <= 16) break;
-        p.block = 16 * p.rb * (p.wt ? kWideWaves / p.wt : 1);
+        p.block = 16 * p.rb * (p.wide ? kWideWaves : 1);
         const long groups = (long)n_seq * kv_heads * ((rows + p.block - 1) / p.block);
         for (int n : kSplits) {
             if (n > 1 && n > tiles) break;
             p.splits = n;
-            const float us = attn_cost(p, D, f32, groups, rows, tiles);
+            const float us = attn_cost(p, D, dtype, groups, rows, tiles);
             if (!best.rb || us < least) {
                 best = p;
                 least = us;
@@ -957,8 +885,7 @@ static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, d
     constexpr bool F32 = DT == QFM_DT_F32;
     constexpr int RB = wide_blocks(D, F32);
     const dim3 b(64 * kAttnWaves), bw(64 * kWideWaves);
-    if (p.wt == 1) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 1>), g, bw, 0, s, v, a);
-    else if (p.wt == 2) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT, 2>), g, bw, 0, s, v, a);
+    if (p.wide) hipLaunchKernelGGL((k_tree_wide<FMT, D, RB, DT>), g, bw, 0, s, v, a);
     else if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, DT>), g, b, 0, s, v, a);
     else if constexpr (few_blocks(D, F32) == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, DT>), g, b, 0, s, v, a);
 }
@@ -993,8 +920,8 @@ extern "C" {
 size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
     if (attn_shape(c, n_seq, T, q_heads, max_nodes, max_ctx)) return 0;
     int splits = 1;
-    for (int f32 = 0; f32 < 2; f32++)
-        splits = max(splits, attn_plan(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, f32).splits);
+    for (int dtype : {QFM_DT_F32, QFM_DT_BF16, QFM_DT_F16})
+        splits = std::max(splits, attn_plan(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, dtype).splits);
     return attn_ws(c, splits, T, q_heads);
 }
 
@@ -1027,7 +954,7 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
     }
     if (!(scale > 0.0f) || !(scale < 3.4e38f)) { set_error(-1, "%s: scale %g", who, (double)scale); return -1; }
     const int D = c->head_dim, G = q_heads / c->kv_heads;
-    const AttnPlan p = attn_plan(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype == QFM_DT_F32);
+    const AttnPlan p = attn_plan(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype);
     const int splits = p.splits;
     const size_t need = attn_ws(c, splits, T, q_heads);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) & 15)) {
