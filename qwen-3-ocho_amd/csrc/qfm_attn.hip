@@ -183,7 +183,10 @@ struct Rows {
                 for (int e = 0; e < 4; e++) {
                     const float p = __builtin_amdgcn_exp2f(fmaf(s[rb][i][e], qs[rb], -m[rb]));
                     l[rb] += p;
-                    const float x = p * vs[i][e];
+                    float x = p * vs[i][e];
+                    // the rounded product, to both uses: the compiler may else round the exact one for the
+                    // first part and take the remainder of the other, a whole fp16 step apart next to a tie
+                    if constexpr (PP == 2) asm("" : "+v"(x));
                     const _Float16 hi = (_Float16)x;
                     pf[rb][0][4 * i + e] = hi;
                     if constexpr (PP == 2) pf[rb][1][4 * i + e] = (_Float16)(x - (float)hi);

@@ -110,6 +110,30 @@ def test_against_64_bits(fmt, dt, counts, ctx, Hq, H, D, page, layout):
     _run(rng, c, counts, ctx, Hq, dt, layout=layout)
 
 
+@pytest.mark.parametrize("fmt", [INT8, E4M3])
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("seqs,m,Hq,H,max_ctx", [
+    (9, 3, 16, 1, 0),                                       # one workgroup a block of rows
+    (3, 17, 8, 8, 5000),                                    # 32 rows a wave, the keys in a few splits
+    (1, 8, 16, 1, 400000),                                  # in as many as there are
+    (3, 64, 32, 2, 8000),                                   # 256 rows and more a head
+    (2, 8, 32, 2, 100000),
+    (33, 17, 8, 8, 1300),
+    (40, 40, 16, 1, 0)])
+def test_every_layout(seqs, m, Hq, H, max_ctx, D, dt, fmt):
+    """The host's bound of the contexts chooses the layout: each form, over short sequences of many lengths (so that
+    splits without keys, waves without rows and sequences of fewer rows than planned are all there)."""
+    _say("fmt", fmt, dt, "D", D, "sequences", seqs, "nodes", m, "heads", Hq, H, "planned for", max_ctx)
+    rng = np.random.default_rng(seqs * m + Hq + D)
+    counts = [m] + [int(x) for x in rng.integers(0, m + 1, seqs - 1)]
+    ctx = [int(x) for x in rng.integers(0, 90, seqs)]
+    if seqs > 2:
+        ctx[1], counts[2] = 0, 1
+    c = _pool(rng, [a + b for a, b in zip(ctx, counts)], 16, H, D, fmt)
+    _run(rng, c, counts, ctx, Hq, dt, max_ctx=max_ctx, max_nodes=m, extra=1)
+
+
 @pytest.mark.parametrize("D,dt", [(128, "bf16"), (256, "f16"), (64, "f32")])
 def test_chain_and_rows_of_no_sequence(D, dt):
     """No masks: a chain. Rows behind the last sequence, and a sequence without rows, are left alone."""
