@@ -19,8 +19,18 @@
 //                 channels in 16 bytes.
 // Codes are widened to fp16 exactly (int8 and E4M3 both fit); a row of Q is
 // scaled to [2^14, 2^15) by a power of two; p times the value's scale is kept
-// within fp16 by a power of two of the largest value scale so far. F32 rows
-// carry Q and P as two fp16 numbers each and take every product twice.
+// within fp16 by a power of two of the largest value scale so far. Q is one fp16
+// number (two for F32 rows: bf16 and fp16 fit one), p one for BF16 rows, whose
+// results are rounded to 2^-8 anyway, and two for F16 and F32.
+//
+// The bound of a large call is its cache: 37 users of 2 to 4 thousand tokens,
+// 124 MB of codes and scales, take 33.7 us (3.7 TB/s, a plain sum over as much
+// memory reads 4.0). Many rows a head are bound by the softmax between the two
+// products, 16 rows by 32 tokens of which cost a wave about as long as their
+// MFMAs (61-node trees of five users, 26 GFLOP: 74 us; k_tree_wide below). Few
+// rows and short contexts are bound by the chain of a launch, the page table,
+// the first tile, a join through LDS and one through memory (1021 tokens: 9.8
+// us); what is there to fill the GPU is the split of the keys.
 #include "qfm_kv.h"
 #include "qfm_mfma.h"
 #include "qfm_internal.h"

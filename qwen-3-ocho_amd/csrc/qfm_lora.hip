@@ -9,7 +9,14 @@
 // the product once for each distinct adapter of its 16 rows and keeps the
 // columns that have it. Neighbours of one prompt share an adapter (one pass); a
 // decode batch has up to 16 (EACH: a workgroup for each, none of which waits
-// for the others). No sorting of rows, no atomics, one writer a value.
+// for the others). No sorting of rows, no atomics, one writer a value. The
+// smallest calls take both products in one launch (k_lora_few).
+//
+// What it has to move is base and y (8 bytes an output and row), x and the
+// adapters in use: 97.5 MB for 2050 rows of K 2048 to 4096 + 512 + 512 outputs at
+// rank 64, of which k_lora_in takes 16.5 us and k_lora_out 28 (3.0 TB/s). A decode
+// batch is bound by the chain launch, slots, A and x, sums, launch, h, B, base
+// (37 rows of 24 adapters, 7 MB: 11.3 us).
 #include "qfm_dev.h"
 #include "qfm_mfma.h"
 #include "qfm_internal.h"
@@ -161,18 +168,65 @@ k_lora_in(LoraArgs a) {
     }
 }
 
+// A row's inner values (of the lanes l16 + 16 g: 8 g .. 8 g + 7 of each 32), whole,
+// as 16-bit numbers; returns what undoes their common factor.
+constexpr int inner_count(int dt) { return dt == QFM_DT_BF16 ? 3 : 2; }
+template <int DT, int KS, int NP>
+__device__ __forceinline__ float inner_parts(const float (&v)[KS][8], u32x4_t (&hp)[KS][NP]) {
+    float sc = 1.0f, back = 1.0f;
+    if constexpr (DT == QFM_DT_F16) {
+        float m = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[s][j]));
+        m = fmaxf(m, __shfl_xor(m, 16));
+        const int k = f16_exp(fmaxf(m, __shfl_xor(m, 32)));
+        sc = exp2i(k);
+        back = exp2i(-k);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float c = v[s][2 * j] * sc, d = v[s][2 * j + 1] * sc;
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                if constexpr (DT == QFM_DT_BF16) {
+                    // cut off after 8 bits, three times: 24 bits, nothing lost
+                    const uint32_t u = pack_bf16_hi(c, d);
+                    hp[s][p][j] = u;
+                    c -= bf16_lo(u);
+                    d -= bf16_hi(u);
+                } else {
+                    const f16x2_t u = {(_Float16)c, (_Float16)d};
+                    hp[s][p][j] = __builtin_bit_cast(uint32_t, u);
+                    c -= (float)u.x;
+                    d -= (float)u.y;
+                }
+            }
+        }
+    return back;
+}
+// 8 columns of a row of B from column k on, those from rank on as zeros
+__device__ __forceinline__ u32x4_t rank_columns(u32x4_t b, int keep) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) b[j] &= keep >= 2 * j + 2 ? ~0u : keep == 2 * j + 1 ? 0xFFFFu : 0u;
+    return b;
+}
+
 constexpr int kLoraOutWaves = 4, kLoraOutTiles = 4;   // tiles of 16 outputs a wave
 
 // blockIdx.y: 256 outputs of one projection (first: the projections' first such
 // block), NB 16-row blocks one after another, so many that all workgroups run
-// at once (a workgroup's first block takes 12 us of 2050 rows' 40, the others 4). B's fragments stay in registers
-// from block to block while the adapter is the same. KS: 32-value steps of the
-// rank.
+// at once: a first block takes about 12 us, from its slots over the adapter to
+// the store, those behind it 4. B's fragments stay in registers from block to
+// block while the adapter is the same. KS: 32-value steps of the rank.
 struct LoraFirst { int v[5]; };
 template <int DT, int KS, bool EACH>
 __global__ void __launch_bounds__(64 * kLoraOutWaves)
 k_lora_out(LoraArgs a, LoraFirst first, int NB) {
-    constexpr int NP = DT == QFM_DT_BF16 ? 3 : 2;
+    constexpr int NP = inner_count(DT);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
     int i = 0;
     while (i < 3 && (int)blockIdx.y >= first.v[i + 1]) i++;
@@ -234,16 +288,12 @@ k_lora_out(LoraArgs a, LoraFirst first, int NB) {
                     const uint16_t *wr = w + (size_t)min(o0 + 16 * q + l16, N - 1) * a.R;
 #pragma unroll
                     for (int s = 0; s < KS; s++) {
-                        const int k = 32 * s + 8 * g, keep = rank - k;  // columns from rank on count as zeros
-                        u32x4_t b = *reinterpret_cast<const u32x4_t *>(wr + min(k, a.R - 8));
-#pragma unroll
-                        for (int j = 0; j < 4; j++) b[j] &= keep >= 2 * j + 2 ? ~0u : keep == 2 * j + 1 ? 0xFFFFu : 0u;
-                        bf[q][s] = b;
+                        const int k = 32 * s + 8 * g;
+                        bf[q][s] = rank_columns(*reinterpret_cast<const u32x4_t *>(wr + min(k, a.R - 8)), rank - k);
                     }
                 }
             }
-            // this row's inner values, whole, as 16-bit numbers
-            float v[KS][8], m = 0.0f;
+            float v[KS][8];
 #pragma unroll
             for (int s = 0; s < KS; s++) {
 #pragma unroll
@@ -252,38 +302,9 @@ k_lora_out(LoraArgs a, LoraFirst first, int NB) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) v[s][j] = h[s][j / 4][j % 4];
                 }
-#pragma unroll
-                for (int j = 0; j < 8; j++) m = fmaxf(m, fabsf(v[s][j]));
-            }
-            float sc = 1.0f, back = 1.0f;
-            if constexpr (DT == QFM_DT_F16) {
-                m = fmaxf(m, __shfl_xor(m, 16));
-                const int k = f16_exp(fmaxf(m, __shfl_xor(m, 32)));
-                sc = exp2i(k);
-                back = exp2i(-k);
             }
             u32x4_t hp[KS][NP];
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    float c = v[s][2 * j] * sc, d = v[s][2 * j + 1] * sc;
-#pragma unroll
-                    for (int p = 0; p < NP; p++) {
-                        if constexpr (DT == QFM_DT_BF16) {
-                            // cut off after 8 bits, three times: 24 bits, nothing lost
-                            const uint32_t u = pack_bf16_hi(c, d);
-                            hp[s][p][j] = u;
-                            c -= bf16_lo(u);
-                            d -= bf16_hi(u);
-                        } else {
-                            const f16x2_t u = {(_Float16)c, (_Float16)d};
-                            hp[s][p][j] = __builtin_bit_cast(uint32_t, u);
-                            c -= (float)u.x;
-                            d -= (float)u.y;
-                        }
-                    }
-                }
+            const float back = inner_parts<DT, KS, NP>(v, hp);
             if (here) factor = a.scale[cur] * back;
 #pragma unroll
             for (int q = 0; q < kLoraOutTiles; q++) {
@@ -333,6 +354,165 @@ k_lora_out(LoraArgs a, LoraFirst first, int NB) {
     }
 }
 
+// Both products in one launch, for few rows and small adapters: 256 outputs of a
+// projection, 16 rows and the blockIdx.z-th of their adapters a workgroup, which
+// finds the inner rows by itself (A is read N / 256 times, from the caches but for
+// the first). Everything that depends on the slots alone (x, A, B, base) is
+// requested together.
+template <int DT, int KS>
+__global__ void __launch_bounds__(64 * kLoraInWaves)
+k_lora_few(LoraArgs a, LoraFirst first) {
+    constexpr int NP = inner_count(DT), RT = 2 * KS, NA = 2 * RT, PART = (NA + 2) * 1024, U = KS == 1 ? 4 : 2;
+    constexpr int TL = 2, LH = 32 * KS + 4, LJ = 16 * TL + 4;             // tiles of 16 outputs a wave
+    __shared__ __attribute__((aligned(16))) uint8_t s_buf[kLoraInWaves * PART];
+    __shared__ __attribute__((aligned(16))) float s_h[16 * LH];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, l16 = lane & 15;
+    const int l8 = lane >> 3, ch = lane & 7, blk = (int)blockIdx.x;
+    int i = 0;
+    while (i < 3 && (int)blockIdx.y >= first.v[i + 1]) i++;
+    const int N = a.rows[i], o0 = (((int)blockIdx.y - first.v[i]) * kLoraInWaves + wave) * (16 * TL);
+    const bool whole = N % 4 == 0;
+    // base, 8 rows of 128 bytes a request
+    const int oc = o0 + 4 * ch;
+    f32x4_t bs[2];
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int tr = 16 * blk + 8 * q + l8;
+        bs[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        if (a.base[i] && tr < a.T && oc < N) {
+            const float *p = a.base[i] + (size_t)tr * N + oc;
+            if (whole) bs[q] = *reinterpret_cast<const f32x4_t *>(p);
+            else bs[q] = f32x4_t{p[0], oc + 1 < N ? p[1] : 0.0f, oc + 2 < N ? p[2] : 0.0f, oc + 3 < N ? p[3] : 0.0f};
+        }
+    }
+    const int e = lora_slot(a, blk, l16);
+    uint32_t left = (uint32_t)__ballot(e >= 0) & 0xFFFFu;
+    int cur = -1;
+    for (int skip = (int)blockIdx.z; left; skip--) {
+        const int c = next_slot(e, left);
+        if (skip == 0) {
+            cur = c;
+            break;
+        }
+    }
+    const bool mine = 16 * blk + l16 < a.T && (e == cur || (e < 0 && blockIdx.z == 0));    // (cur -1: those without)
+    const uint32_t rows = (uint32_t)__ballot(mine) & 0xFFFFu;
+    if (!rows || (cur < 0 && blockIdx.z)) return;            // the same for every wave
+    f32x4_t acc[TL];
+#pragma unroll
+    for (int q = 0; q < TL; q++) acc[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float factor = 0.0f;
+    if (cur >= 0) {
+        const int rank = min(max(a.rank[cur], 0), a.R);
+        const float scale = a.scale[cur];
+        u32x4_t bf[TL][KS];
+#pragma unroll
+        for (int q = 0; q < TL; q++)
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                bf[q][s] = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(a.b[i]) +
+                                                              ((size_t)cur * N + min(o0 + 16 * q + l16, N - 1)) * a.R + min(32 * s + 8 * g, a.R - 8));
+        uint8_t *s_w = s_buf + wave * PART, *s_x = s_w + NA * 1024;
+        const uint16_t *x[2], *w[NA];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+            x[n] = static_cast<const uint16_t *>(a.x) + (size_t)min(16 * blk + 8 * n + l8, a.T - 1) * a.xs + 8 * ch;
+#pragma unroll
+        for (int n = 0; n < NA; n++)
+            w[n] = static_cast<const uint16_t *>(a.a[i]) + ((size_t)cur * a.R + min(8 * n + l8, a.R - 1)) * a.K + 8 * ch;
+        f32x4_t h[RT];
+#pragma unroll
+        for (int q = 0; q < RT; q++) h[q] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        const int chunks = a.K / 64;
+        for (int k0 = wave; k0 < chunks; k0 += U * kLoraInWaves) {
+            u32x4_t wv[U][NA], xv[U][2];
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                const size_t at = 64 * (size_t)min(k0 + v * kLoraInWaves, chunks - 1);
+#pragma unroll
+                for (int n = 0; n < NA; n++) wv[v][n] = *reinterpret_cast<const u32x4_t *>(w[n] + at);
+#pragma unroll
+                for (int n = 0; n < 2; n++) xv[v][n] = *reinterpret_cast<const u32x4_t *>(x[n] + at);
+            }
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+                if (k0 + v * kLoraInWaves >= chunks) break;
+#pragma unroll
+                for (int n = 0; n < NA; n++) *reinterpret_cast<u32x4_t *>(s_w + lds_at<128>(8 * n + l8, ch)) = wv[v][n];
+#pragma unroll
+                for (int n = 0; n < 2; n++) *reinterpret_cast<u32x4_t *>(s_x + lds_at<128>(8 * n + l8, ch)) = xv[v][n];
+                wave_lds_fence();
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const u32x4_t xf = *reinterpret_cast<const u32x4_t *>(s_x + lds_at<128>(l16, 4 * j + g));
+#pragma unroll
+                    for (int q = 0; q < RT; q++)
+                        h[q] = lora_mfma<DT>(*reinterpret_cast<const u32x4_t *>(s_w + lds_at<128>(16 * q + l16, 4 * j + g)), xf, h[q]);
+                }
+                wave_lds_fence();
+            }
+        }
+        // the waves' sums meet: lane (g, l16) holds inner values 4 g .. of row l16
+        f32x4_t *s_acc = reinterpret_cast<f32x4_t *>(s_buf);
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < RT; q++) s_acc[(wave * RT + q) * 64 + lane] = h[q];
+        __syncthreads();
+        if (wave < RT) {
+            f32x4_t sum = s_acc[wave * 64 + lane];
+#pragma unroll
+            for (int v = 1; v < kLoraInWaves; v++) sum += s_acc[(v * RT + wave) * 64 + lane];
+            const int r = 16 * wave + 4 * g;
+            *reinterpret_cast<float4 *>(&s_h[l16 * LH + r]) = make_float4(r + 0 < rank ? sum[0] : 0.0f, r + 1 < rank ? sum[1] : 0.0f,
+                                                                          r + 2 < rank ? sum[2] : 0.0f, r + 3 < rank ? sum[3] : 0.0f);
+        }
+        __syncthreads();
+        float v[KS][8];
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float4 y = *reinterpret_cast<const float4 *>(&s_h[l16 * LH + 32 * s + 8 * g + 4 * j]);
+                v[s][4 * j] = y.x; v[s][4 * j + 1] = y.y; v[s][4 * j + 2] = y.z; v[s][4 * j + 3] = y.w;
+            }
+        u32x4_t hp[KS][NP];
+        factor = inner_parts<DT, KS, NP>(v, hp) * scale;
+#pragma unroll
+        for (int q = 0; q < TL; q++) {
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                const u32x4_t b = rank_columns(bf[q][s], rank - (32 * s + 8 * g));
+#pragma unroll
+                for (int p = 0; p < NP; p++) acc[q] = lora_mfma<DT>(b, hp[s][p], acc[q]);
+            }
+            // chosen: the columns of rows with other adapters hold what is none of theirs
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[q][j] = e == cur ? factor * acc[q][j] : 0.0f;
+        }
+    }
+    float *sy = reinterpret_cast<float *>(s_buf) + wave * (16 * LJ);
+#pragma unroll
+    for (int q = 0; q < TL; q++)
+        *reinterpret_cast<float4 *>(&sy[l16 * LJ + 16 * q + 4 * g]) = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+    wave_lds_fence();
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+        const int r = 8 * q + l8;
+        const float4 d = *reinterpret_cast<const float4 *>(&sy[r * LJ + 4 * ch]);
+        if (!(rows >> r & 1) || oc >= N) continue;
+        const float4 v = make_float4(bs[q][0] + d.x, bs[q][1] + d.y, bs[q][2] + d.z, bs[q][3] + d.w);
+        float *y = a.y[i] + (size_t)(16 * blk + r) * N + oc;
+        if (whole) {
+            *reinterpret_cast<float4 *>(y) = v;
+        } else {
+            y[0] = v.x;
+            if (oc + 1 < N) y[1] = v.y;
+            if (oc + 2 < N) y[2] = v.z;
+            if (oc + 3 < N) y[3] = v.w;
+        }
+    }
+}
+
 // up to here a workgroup for each of a block's up to 16 adapters
 constexpr int kLoraEachRows = 256;
 
@@ -347,10 +527,28 @@ static int lora_check(const qfm_lora *l, int T, const char *who) {
     return 0;
 }
 
+// k_lora_few rather than two launches: while its workgroups, with A once each, are
+// no more than the CUs, and A is short enough to arrive in two rounds of loads.
+// One row to 4096 + 512 + 512 outputs of K 2048, rank 16: 6.2 us, 8.7 with two; 16
+// rows of 16 adapters, 2560 of 2560, rank 32: 9.2 and 12.1; but 37 rows of that
+// 16.3 and 12.5, one row of K 8192, rank 64, 18.3 and 13.3.
+static bool lora_few(const LoraArgs &a, int outs) {
+    const int each = a.T < 16 ? a.T : 16;
+    return a.R <= 64 && a.K <= 4096 && a.R * a.K <= 1 << 17 && (long)((a.T + 15) / 16) * (each < a.slots ? each : a.slots) * outs <= 256;
+}
+
 template <int DT, bool EACH>
 static void lora_launch(const LoraArgs &a, const LoraFirst &f, hipStream_t s) {
     constexpr int RT = EACH ? 1 : 4, CB = EACH ? 1 : 2;
     const int blocks = (a.T + 15) / 16, tiles = a.n * ((a.R + 15) / 16);
+    if constexpr (EACH) {
+        if (lora_few(a, f.v[4])) {
+            const dim3 g((unsigned)blocks, (unsigned)f.v[4], 16u), b(64 * kLoraInWaves);
+            if (a.R <= 32) hipLaunchKernelGGL((k_lora_few<DT, 1>), g, b, 0, s, a, f);
+            else hipLaunchKernelGGL((k_lora_few<DT, 2>), g, b, 0, s, a, f);
+            return;
+        }
+    }
     hipLaunchKernelGGL((k_lora_in<DT, RT, CB>), dim3((unsigned)((blocks + CB - 1) / CB), (unsigned)((tiles + RT - 1) / RT), EACH ? 16u : 2u),
                        dim3(64 * kLoraInWaves), 0, s, a);
     const int nb = EACH ? 1 : (int)(((long)blocks * f.v[4] + 511) / 512);

@@ -94,7 +94,10 @@ class Case:
     (1, 1, 8, 64, [1], "any"), (1, 5, 16, 2048, [4096, 512, 512], "any"), (8, 3, 16, 2560, [640, 640], "any"),
     (37, 24, 32, 512, [1021], "any"), (16, 16, 128, 128, [256], "each"), (17, 4, 24, 320, [63, 64, 65, 2], "any"),
     (256, 9, 64, 192, [130], "any"), (257, 9, 64, 192, [130], "any"), (700, 6, 40, 256, [512, 33], "runs"),
-    (530, 40, 8, 64, [100], "any"), (300, 2, 128, 1024, [128], "runs")])
+    (530, 40, 8, 64, [100], "any"), (300, 2, 128, 1024, [128], "runs"),
+    # both products in one launch: ranks and K at its ends, ragged rows and outputs, and one beyond each bound
+    (16, 5, 64, 2048, [33], "any"), (37, 24, 8, 64, [255, 2], "any"), (5, 2, 40, 3200, [600], "any"), (1, 1, 24, 4096, [7, 300], "any"),
+    (250, 2, 16, 576, [256, 256], "any"), (3, 3, 72, 512, [64], "each"), (2, 2, 64, 2112, [64], "each"), (2, 9, 8, 4160, [64], "each")])
 def test_against_64_bits(dt, T, slots, R, K, ns, kind):
     _say(dt, "rows", T, "slots", slots, "R", R, "K", K, "outputs", ns, kind)
     rng = np.random.default_rng(T * 31 + R + K)
