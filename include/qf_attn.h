@@ -85,8 +85,9 @@ int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, 
  *   out(t, h) = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q(t, h) . k_j - max)
  * over the positions that row t sees, with the keys and values of head
  * h / (q_heads / kv_heads). A row that sees nothing gets zeros. Scores, maxima,
- * sums and results are held in fp32; q and p enter the products as fp16 scaled
- * by powers of two (F32 rows: as two fp16 numbers, 22 bits), the codes exactly.
+ * sums and results are held in fp32. Q and p times the value's scale enter the
+ * products as fp16 scaled by powers of two, the codes exactly: q as one number
+ * (F32 rows: two, 22 bits), p as one for BF16 rows and two for F16 and F32.
  *   q, out  element (t, h, d) at t * row_stride + h * head_stride + d, type
  *           dtype; strides multiples of 8 and not negative (out: at least D),
  *           16-byte aligned. Rows of out that no sequence has are left.
