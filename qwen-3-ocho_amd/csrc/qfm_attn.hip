@@ -617,10 +617,16 @@ k_tree_wide(KvView c, AttnArgs a) {
     R.clear();
     if (t0 < t1) widen(t0, pc);
     if (t0 + 1 < t1) request(t0 + 1, pn);
-    __syncthreads();
-    for (int t = t0; t < t1; t++) {
+    // the next tile: half of the waves widen their part of it before this tile's
+    // products and half behind them, so that the two waves of a SIMD are not both at
+    // their conversions and both at their MFMAs (61-node trees 75.2 -> 73.2 us)
+    auto ahead = [&](int t) {
         if (t + 1 < t1) widen(t + 1, pn);
         if (t + 2 < t1) request(t + 2, pf2);
+    };
+    __syncthreads();
+    for (int t = t0; t < t1; t++) {
+        if (wave < kWideWaves / 2) ahead(t);
         if (live) {
             const uint8_t *buf = s_buf + (t & 1) * (TILES / 2) + lane * 16;
             f32x4_t s[RB][2];
@@ -670,6 +676,7 @@ k_tree_wide(KvView c, AttnArgs a) {
                         for (int rb = 0; rb < RB; rb++) R.o[rb][k][q] = mfma_f16(vf, pf[rb][n], R.o[rb][k][q]);
                 }
         }
+        if (wave >= kWideWaves / 2) ahead(t);
         pc = pn;
         pn = pf2;
         pf2 = pages(t + 3);
