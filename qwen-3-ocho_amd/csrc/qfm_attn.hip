@@ -27,7 +27,7 @@
 // 124 MB of codes and scales, take 33.7 us (3.7 TB/s, a plain sum over as much
 // memory reads 4.0). Many rows a head are bound by the softmax between the two
 // products, 16 rows by 32 tokens of which cost a wave about as long as their
-// MFMAs (61-node trees of five users, 26 GFLOP: 74 us; k_tree_wide below). Few
+// MFMAs (61-node trees of five users, 26 GFLOP: 71 us; k_tree_wide below). Few
 // rows and short contexts are bound by the chain of a launch, the page table,
 // the first tile, a join through LDS and one through memory (1021 tokens: 9.8
 // us); what is there to fill the GPU is the split of the keys.
@@ -836,7 +836,7 @@ constexpr int few_resident(int D, int rb) { return rb == 1 ? (D == 64 ? 3 : 2) :
 // What it picks takes 1.3% more than the best layout on average; one round of
 // resident workgroups with the widest rows took 22% more. Each form is there for
 // what the others lose without it: 16 rows a wave 17%, 32 rows 4%, k_tree_wide 3%
-// (61-node trees of five users: 84 us, 75 with it).
+// (61-node trees of five users: 84 us, 75 with it before its waves were offset).
 static float attn_cost(const AttnPlan &p, int D, int dtype, long groups, int rows, long tiles) {
     const float d = D / 128.0f, each = p.wide ? 1 : kAttnWaves;
     const bool f32 = dtype == QFM_DT_F32, f16 = dtype == QFM_DT_F16;

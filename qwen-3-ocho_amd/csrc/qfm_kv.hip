@@ -3,8 +3,9 @@
 //
 // A row of one head is D values with one scale: amax over the row, then one
 // quotient a value. Both kernels are bound by bytes (2 or 4 in and 1 out a
-// value, or the reverse) and, at a few rows, by the chain of dependent loads
-// row -> sequence and position -> page.
+// value, or the reverse: 8038 rows of 8 x 128 in 13.8 us written, 11.9 read,
+// 50 MB at 3.6 and 4.2 TB/s) and, at a few rows, by the chain of dependent loads
+// row -> sequence and position -> page (3.3 us alone; a call costs the host 4).
 #include "qfm_kv.h"
 #include "qfm_internal.h"
 
@@ -98,7 +99,7 @@ __device__ __forceinline__ uint32_t transpose_rows(uint32_t x, int r) {
 
 // Few rows (up to kFewRows): what counts is the chain row -> place -> stores, so
 // keys and values are rows of their own, 8 values a lane, every value code a byte
-// store (8 rows of 2 x 256: 4.4 us a call, 5.4 in fours as below).
+// store (8 rows of 2 x 256: 4.2 us a call, 5.4 in fours as below).
 constexpr int kFewRows = 64;
 template <int DT, int FMT, int D>
 __global__ void __launch_bounds__(kKvThreads)
