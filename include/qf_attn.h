@@ -42,7 +42,7 @@ extern "C" {
  *      side by side, so that attention's second product, whose inner dimension
  *      is the tokens, loads its operand as it lies
  *   ks, vs  fp32 scales [n_pages][kv_heads][page]
- * k and v 16-byte aligned. Pages need no initialisation. */
+ * k, v, ks and vs 16-byte aligned. Pages need no initialisation. */
 typedef struct {
     void  *k, *v;
     float *ks, *vs;
@@ -84,7 +84,8 @@ int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, 
  * is max_nodes 1, its mask 1 or NULL.
  *   out(t, h) = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q(t, h) . k_j - max)
  * over the positions that row t sees, with the keys and values of head
- * h / (q_heads / kv_heads). A row that sees nothing gets zeros. Scores, maxima,
+ * h / (q_heads / kv_heads). A row that sees nothing gets zeros; a row of q that
+ * is not finite gets NaN. Of a sequence's positions the first 2^31 - 2^16 are seen. Scores, maxima,
  * sums and results are held in fp32. Q and p times the value's scale enter the
  * products as fp16 scaled by powers of two, the codes exactly: q as one number
  * (F32 rows: two, 22 bits), p as one for BF16 rows and two for F16 and F32.

@@ -44,7 +44,8 @@ int  qf8_i8_gemv_rows(const Qf8I8Multi *mm, const int8_t *xq, const float *xs, i
  * int32); a row whose slot is not in [0, slots) has no adapter: y = base. base[i]
  * and y[i] are fp32 [T][rows[i]]; base[i] may be y[i] (added in place) or NULL
  * (zeros). The inner row a x is held in fp32 and enters the second product
- * whole (three bf16 numbers, or two fp16 ones scaled by a power of two).
+ * whole (three bf16 numbers, or two fp16 ones scaled by a power of two); where
+ * it is infinite, y is NaN. Rows affect no other rows.
  * 1 <= n <= 4; K a multiple of 64 up to 65536; R a multiple of 8 up to 128;
  * T up to 2^20; x, a, b, base and y 16-byte aligned, x_stride a multiple of 8
  * and not negative. No counterpart in the reference. */

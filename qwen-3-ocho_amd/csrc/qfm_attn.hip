@@ -232,8 +232,10 @@ struct QRow {
 #pragma unroll
                 for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(v[k][j][e]));
             }
-        const int k2 = f16_exp(max_over_g(m));
-        const float sc = exp2i(k2);
+        const float top = max_over_g(m);
+        const int k2 = f16_exp(top);
+        // a row with an infinity is NaN wherever it sees a key, also where every score would be -infinity
+        const float sc = top < INFINITY ? exp2i(k2) : NAN;
 #pragma unroll
         for (int k = 0; k < NC; k++)
 #pragma unroll

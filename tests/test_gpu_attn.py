@@ -173,6 +173,27 @@ def test_rows_lost_to_nan_reach_only_those_that_see_them(fmt):
         assert np.isnan(want[2:4]).all() and np.isfinite(np.delete(want, [2, 3], 0)).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+def test_queries_that_are_not_finite(dt):
+    """An infinity or a NaN in a row of q: NaN for that row and head alone, whatever the signs of its keys; zeros where it
+    sees nothing."""
+    rng = np.random.default_rng(18)
+    for counts, ctx, tree in (([3], [0], [1, 2, 0]), ([5, 40], [33, 200], None)):
+        T, Hq, H, D = sum(counts), 4, 1, 64
+        c = _pool(rng, [a + b for a, b in zip(ctx, counts)], 16, H, D, INT8)
+        c.k[:, :, :, 7] = 0x85                                          # one channel negative in every key
+        x = rng.standard_normal((T, Hq, D)).astype(np.float32)
+        x[0, 0, 7], x[1, 1, 9], x[1, 2, 7], x[2, 3, 3] = np.inf, -np.inf, np.nan, np.inf
+        bits, q = _kv.to_dtype(x, dt)
+        tree = None if tree is None else np.array(tree, np.uint64)
+        call = Call(c, bits, dt, counts, ctx, tree, D ** -0.5)
+        call()
+        with np.errstate(invalid="ignore"):
+            want, tol = _kv.attention(c, q, np.cumsum([0] + counts), ctx, tree, np.float32(D ** -0.5), dt)
+        assert np.isnan(want[0, 0]).all() and np.isfinite(want[0, 1:]).all()
+        _check(call.result(), dt, want, tol, call.fill)
+
+
 @pytest.mark.parametrize("fmt", [INT8, E4M3])
 def test_pages_that_do_not_exist_are_not_seen(fmt):
     rng = np.random.default_rng(12)
