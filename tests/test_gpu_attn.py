@@ -260,6 +260,41 @@ def test_replays_with_growing_contexts():
     assert lib.qfm_graph_destroy(g) == 0
 
 
+def test_two_graphs_share_a_workspace():
+    """Two captured calls of different shapes on one workspace, replayed in turn on one stream: each as by itself."""
+    rng, lib = np.random.default_rng(19), qfm.load()
+    calls, want = [], []
+    for counts, ctx, Hq, H, D, dt in (([3, 1], [900, 40], 8, 2, 128, "bf16"), ([20], [2100], 16, 2, 64, "f32")):
+        c = _pool(rng, [a + b for a, b in zip(ctx, counts)], 32, H, D, INT8)
+        bits, q = _kv.to_dtype(rng.standard_normal((sum(counts), Hq, D)).astype(np.float32), dt)
+        calls.append(Call(c, bits, dt, counts, ctx, None, D ** -0.5))
+        want.append(_kv.attention(c, q, np.cumsum([0] + counts), ctx, None, np.float32(D ** -0.5), dt))
+    sizes = [c.args[-1] for c in calls]
+    assert min(sizes) > 0
+    ws, st = qfm.DevBuf.from_array(np.full(max(sizes), 0xFF, np.uint8)), calls[0].st
+    graphs = []
+    for c, size in zip(calls, sizes):
+        c.args, c.st = (*c.args[:-2], ws.ptr, size), st
+        qfm.check(lib.qfm_graph_capture_begin(st.h), "capture")
+        c()
+        graphs.append(lib.qfm_graph_capture_end(st.h))
+        assert graphs[-1], lib.qfm_last_error().decode()
+    first = None
+    for rep in range(4):
+        for c in calls:
+            c.b["out"].upload(np.full(c.n, c.fill, _kv.NP[c.dt]))
+        for g in graphs:
+            qfm.check(lib.qfm_graph_launch(g, st.h), "launch")
+        got = [c.result() for c in calls]
+        for c, y, (w, tol) in zip(calls, got, want):
+            _check(y, c.dt, w, tol, c.fill)
+        assert first is None or all(np.array_equal(a, b) for a, b in zip(got, first))
+        first = got
+        calls[rep % 2]()                                                # an eager one on the same workspace between
+    for g in graphs:
+        assert lib.qfm_graph_destroy(g) == 0
+
+
 def test_pages_behind_four_gigabytes():
     rng, lib = np.random.default_rng(16), qfm.load()
     page, H, D, pages, ctx, m, Hq = 256, 8, 256, 8300, 300, 2, 8
