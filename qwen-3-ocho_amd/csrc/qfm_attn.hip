@@ -24,10 +24,10 @@
 // results are rounded to 2^-8 anyway, and two for F16 and F32.
 //
 // The bound of a large call is its cache: 37 users of 2 to 4 thousand tokens,
-// 124 MB of codes and scales, take 33.7 us (3.7 TB/s, a plain sum over as much
+// 124 MB of codes and scales, take 33.0 us (3.8 TB/s, a plain sum over as much
 // memory reads 4.0). Many rows a head are bound by the softmax between the two
 // products, 16 rows by 32 tokens of which cost a wave about as long as their
-// MFMAs (61-node trees of five users, 26 GFLOP: 71 us; k_tree_wide below). Few
+// MFMAs (61-node trees of five users, 26 GFLOP: 64 us; k_tree_wide below). Few
 // rows and short contexts are bound by the chain of a launch, the page table,
 // the first tile, a join through LDS and one through memory (1021 tokens: 9.8
 // us); what is there to fill the GPU is the split of the keys.
@@ -48,19 +48,162 @@ constexpr int kVeMin = -118;       // least exponent of the value scale that the
 struct AttnArgs {
     const uint8_t *q;
     uint8_t *out;
-    int G, T, max_nodes, splits;
+    int G, T, max_nodes, splits;   // splits: 1, or workgroups a sequence on average
+    int dealt, rows;               // rows: what po and pml have room for
     long qrs, qhs, ors, ohs;
     const int *row_start, *ctx;
     const uint64_t *tree;
     float scale;
-    float *po;                     // [splits][T][q_heads][D], normalised
-    float2 *pml;                   // [splits][T][q_heads] {maximum (base 2), sum}
+    float *po;                     // [rows][q_heads][D], normalised
+    float2 *pml;                   // [rows][q_heads] {maximum (base 2), sum}
+    int2 *parts;                   // [n_seq] {splits, first row of po and pml}
 };
 
 // the rows of sequence s: first row, count
 __device__ __forceinline__ int2 seq_rows(const int *row_start, int s, int T, int max_nodes) {
     const int r0 = row_start[s], r1 = min(row_start[s + 1], T);
     return make_int2(r0, r0 < 0 || r1 <= r0 ? 0 : min(r1 - r0, max_nodes));
+}
+
+// inclusive sums over the lanes
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);      // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+// sum and maximum (of values from 0 on) over the lanes, as scalars
+__device__ __forceinline__ int wave_add(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_top(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// A workgroup's share: tiles t0 .. t1 - 1 of sequence seq (rows r0 .. r0 + m - 1,
+// ctx tokens before them, len with them), which is split n ways; row: its first
+// row of the partial results, first: that of the sequence. m = 0: nothing.
+struct Share { int seq, r0, m, ctx, len, t0, t1, n, row, first; };
+constexpr int kDealSeqs = 256;     // four a lane
+// Sequences differ in length, so the workgroups along x are dealt out by tiles:
+// chunks of as few tiles as still give every chunk a workgroup, found by bisection
+// between total / workgroups and what is enough whatever the remainders (a chunk
+// at most 1/8 of that range longer than need be). Every wave works this out for
+// itself from all the lengths, one to four a lane: about 1 us of a call (16 users
+// of 4000 tokens 31.9 -> 33.4), for which 61-node trees of five users take 64 us
+// instead of 71 and one user of 131071 tokens among 36 of 1000 64 instead of 231.
+__device__ __forceinline__ Share share_of(const KvView &c, const AttnArgs &a, int lane) {
+    const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
+    Share w{};
+    int nt, per, j;
+    if (!a.dealt) {
+        w.seq = (int)blockIdx.z;
+        const int2 sr = seq_rows(a.row_start, w.seq, a.T, a.max_nodes);
+        w.r0 = sr.x;
+        w.m = sr.y;
+        w.ctx = (int)min((long)max(a.ctx[w.seq], 0), cap);
+        w.n = a.splits;
+        j = (int)blockIdx.x;
+        nt = ((int)min((long)w.ctx + w.m, cap) + 31) >> 5;
+        per = (nt + w.n - 1) / w.n;
+        w.row = w.n * w.r0;
+    } else {
+        constexpr int Q = kDealSeqs / 64;
+        const int slots = (int)gridDim.x, slot = (int)blockIdx.x;
+        int r0[Q], m[Q], ctx[Q], tiles[Q], total = 0, most = 0, have = 0;
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            r0[q] = m[q] = ctx[q] = tiles[q] = 0;
+            if (64 * q < c.n_seq) {
+                const int s = min(64 * q + lane, c.n_seq - 1);
+                const int2 sr = seq_rows(a.row_start, s, a.T, a.max_nodes);
+                r0[q] = sr.x;
+                m[q] = 64 * q + lane < c.n_seq ? sr.y : 0;
+                ctx[q] = (int)min((long)max(a.ctx[s], 0), cap);
+                tiles[q] = m[q] ? ((int)min((long)ctx[q] + m[q], cap) + 31) >> 5 : 0;
+                total += tiles[q];
+                most = max(most, tiles[q]);
+                have += (int)__popcll(__ballot(tiles[q] > 0));
+            }
+        }
+        total = wave_add(total);
+        most = wave_top(most);
+        // lo from below and hi from above by more than the roundings of their quotients (slots > sequences)
+        int lo = max(max(1, (int)((float)total * __builtin_amdgcn_rcpf((float)slots) * (1.0f - 0x1p-20f))), (most + kMaxSplits - 1) / kMaxSplits);
+        int hi = max(lo, (int)((float)total * __builtin_amdgcn_rcpf((float)(slots - have)) * (1.0f + 0x1p-20f)) + 1);
+        int n[Q], mid = hi;
+        // n: tiles in chunks of mid, rounded up; at most kMaxSplits, so that the fp32 quotient is off by one at most
+        const auto chunks = [&]() {
+            const float inv = __builtin_amdgcn_rcpf((float)mid);
+            int sum = 0;
+#pragma unroll
+            for (int q = 0; q < Q; q++)
+                if (64 * q < c.n_seq) {
+                    const int f = (int)((float)tiles[q] * inv), rest = tiles[q] - f * mid;
+                    n[q] = f + (rest > 0) + (rest > mid);
+                    sum += n[q];
+                }
+            return sum;
+        };
+        for (int i = 0; i < 3 && lo < hi; i++) {
+            mid = (lo + hi) >> 1;
+            if (wave_add(chunks()) <= slots) hi = mid;
+            else lo = mid + 1;
+        }
+        mid = per = __builtin_amdgcn_readfirstlane(hi);
+        chunks();
+        nt = j = 0;
+        int before = 0, rows = 0;                              // workgroups and rows of the sequences before
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (64 * q < c.n_seq) {
+                const int upto = before + wave_scan(n[q]), r = rows + wave_scan(n[q] * m[q]);
+                const uint64_t hit = __ballot(slot < upto && slot >= upto - n[q]);
+                if (hit) {
+                    const int l = __builtin_ctzll(hit);
+                    w.seq = 64 * q + l;
+                    w.r0 = __builtin_amdgcn_readlane(r0[q], l);
+                    w.m = __builtin_amdgcn_readlane(m[q], l);
+                    w.ctx = __builtin_amdgcn_readlane(ctx[q], l);
+                    w.n = __builtin_amdgcn_readlane(n[q], l);
+                    nt = __builtin_amdgcn_readlane(tiles[q], l);
+                    j = slot - __builtin_amdgcn_readlane(upto - n[q], l);
+                    w.row = __builtin_amdgcn_readlane(r - n[q] * m[q], l);
+                }
+                before = __builtin_amdgcn_readlane(upto, 63);
+                rows = __builtin_amdgcn_readlane(r, 63);
+            }
+    }
+    w.len = (int)min((long)w.ctx + w.m, cap);
+    w.t0 = j * per;
+    w.t1 = min(nt, w.t0 + per);
+    // ranges of rows that overlap would need more room than there is: no share
+    if (w.n > 1 && (w.row < 0 || w.row + w.n * w.m > a.rows)) w.m = 0;
+    w.first = w.row;
+    w.row += j * w.m;
+    return w;
+}
+// what the joins need to know. Behind the loop: a store ahead of it would have the
+// page table read through the vector cache, tile by tile behind the keys (61-node
+// trees 88 us for 73)
+__device__ __forceinline__ void put_parts(const AttnArgs &a, const Share &w) {
+    if (a.dealt && blockIdx.y == 0 && w.row == w.first && threadIdx.x == 0) a.parts[w.seq] = make_int2(w.n, w.first);
+}
+// for the joins: a sequence's splits and first row, 0 splits for none or for
+// results that are in place already
+template <bool DEALT>
+__device__ __forceinline__ int2 parts_of(const AttnArgs &a, int seq, int2 sr) {
+    if constexpr (!DEALT) return make_int2(a.splits, a.splits * sr.x);
+    const int2 p = a.parts[seq];
+    const bool right = sr.y > 0 && p.x > 1 && p.x <= kMaxSplits && p.y >= 0 && p.y <= a.rows && p.x * sr.y <= a.rows - p.y;
+    return make_int2(right ? p.x : 0, p.y);
 }
 
 template <int FMT>
@@ -273,18 +416,15 @@ k_tree_attn(KvView c, AttnArgs a) {
     __shared__ int s_ve[kAttnWaves];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int g = lane >> 4, l16 = lane & 15;
-    const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
-    const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
-    const int rows = sr.y * a.G, row0 = blk * ROWS;
+    const int h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
+    const Share w = share_of(c, a, lane);
+    const int rows = w.m * a.G, row0 = blk * ROWS;
     if (row0 >= rows) return;
-    const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
-    const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
-    const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
-    const int t1 = min(nt, ((int)blockIdx.x + 1) * per);
-    int t = (int)blockIdx.x * per + wave;
+    const int ctx = w.ctx, len = w.len, t1 = w.t1;
+    int t = w.t0 + wave;
 
     // the pages of a tile's halves (-1: none), requested a tile ahead; loads from page 0 in place of none
-    const int *table = c.table + (size_t)seq * c.max_pages;
+    const int *table = c.table + (size_t)w.seq * c.max_pages;
     auto pages = [&](int tt) {
         const int p = 32 * tt, last = c.max_pages - 1;
         int x = table[min(p >> c.page_log2, last)], y = table[min((p + 16) >> c.page_log2, last)];
@@ -325,8 +465,8 @@ k_tree_attn(KvView c, AttnArgs a) {
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         const int r = min(row0 + 16 * rb + l16, rows - 1), node = r / a.G;
-        if ((rb & (kAttnWaves - 1)) == wave) q[rb].load(a, sr.x, h, r, node, g);
-        R.see[rb] = node_mask(a, sr.x, node);
+        if ((rb & (kAttnWaves - 1)) == wave) q[rb].load(a, w.r0, h, r, node, g);
+        R.see[rb] = node_mask(a, w.r0, node);
     }
     Tile<NC> kt[DEEP ? 2 : 1], vt[DEEP ? 2 : 1];
     int2 pg = pages(t);
@@ -456,6 +596,7 @@ k_tree_attn(KvView c, AttnArgs a) {
         }
     }
 
+    put_parts(a, w);
     // join the waves
     __syncthreads();                       // Q has been read
 #pragma unroll
@@ -504,11 +645,10 @@ k_tree_attn(KvView c, AttnArgs a) {
         const float inv = sum == 0.0f ? 0.0f : back / sum;
         x.x *= inv; x.y *= inv; x.z *= inv; x.w *= inv;
         const int node = (row0 + r) / a.G, head = h * a.G + (row0 + r) - node * a.G;
-        const long t = sr.x + node;
-        if (a.splits == 1) {
-            store4<DT>(a.out, t * a.ors + head * a.ohs + d, x);
+        if (w.n == 1) {
+            store4<DT>(a.out, (w.r0 + node) * a.ors + head * a.ohs + d, x);
         } else {
-            const size_t at = ((size_t)blockIdx.x * a.T + t) * heads + head;
+            const size_t at = (size_t)(w.row + node) * heads + head;
             *reinterpret_cast<float4 *>(a.po + at * D + d) = x;
             if (d == 0) a.pml[at] = make_float2(mn, sum);
         }
@@ -533,18 +673,15 @@ k_tree_wide(KvView c, AttnArgs a) {
     __shared__ float s_sc[2][64];                           // 32 key scales, 32 value scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int g = lane >> 4, l16 = lane & 15;
-    const int seq = (int)blockIdx.z, h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
-    const int2 sr = seq_rows(a.row_start, seq, a.T, a.max_nodes);
-    const int rows = sr.y * a.G, row0 = blk * ROWS;
+    const int h = (int)blockIdx.y % c.heads, blk = (int)blockIdx.y / c.heads;
+    const Share w = share_of(c, a, lane);
+    const int rows = w.m * a.G, row0 = blk * ROWS;
     if (row0 >= rows) return;
-    const long cap = min((long)c.max_pages << c.page_log2, kMaxTokens);
-    const int ctx = (int)min((long)max(a.ctx[seq], 0), cap), len = (int)min((long)ctx + sr.y, cap);
-    const int nt = (len + 31) >> 5, per = (nt + a.splits - 1) / a.splits;
-    const int t0 = (int)blockIdx.x * per, t1 = min(nt, t0 + per);
+    const int ctx = w.ctx, len = w.len, t0 = w.t0, t1 = w.t1;
     const int lim = min(len, 32 * t1);                      // tokens from here on are no keys of this workgroup
     const bool live = row0 + 16 * RB * wave < rows;           // this wave has rows
 
-    const int *table = c.table + (size_t)seq * c.max_pages;
+    const int *table = c.table + (size_t)w.seq * c.max_pages;
     auto pages = [&](int tt) {
         const int p = 32 * tt, last = c.max_pages - 1;
         int x = table[min(p >> c.page_log2, last)], y = table[min((p + 16) >> c.page_log2, last)];
@@ -608,8 +745,8 @@ k_tree_wide(KvView c, AttnArgs a) {
 #pragma unroll
     for (int rb = 0; rb < RB; rb++) {
         const int r = min(row0 + 16 * (RB * wave + rb) + l16, rows - 1), node = r / a.G;
-        q[rb].load(a, sr.x, h, r, node, g);
-        R.see[rb] = node_mask(a, sr.x, node);
+        q[rb].load(a, w.r0, h, r, node, g);
+        R.see[rb] = node_mask(a, w.r0, node);
     }
     int2 pc = pages(t0), pn = pages(t0 + 1), pf2 = pages(t0 + 2);   // of this tile and the next two
     if (t0 < t1) request(t0, pc);
@@ -685,16 +822,17 @@ k_tree_wide(KvView c, AttnArgs a) {
         __syncthreads();
     }
 
+    put_parts(a, w);
     // 4 channels of a row, to the results or the workspace; 64 channels of a row
     // a turn, brought side by side through LDS
     const int heads = c.heads * a.G;
     struct Place { long t; int head; size_t at; };
     auto place = [&](int r) {
         const int node = r / a.G, head = h * a.G + r - node * a.G;
-        return Place{sr.x + node, head, ((size_t)blockIdx.x * a.T + sr.x + node) * heads + head};
+        return Place{w.r0 + node, head, (size_t)(w.row + node) * heads + head};
     };
     auto put = [&](const Place &p, int d, float4 x) {
-        if (a.splits == 1) store4<DT>(a.out, p.t * a.ors + p.head * a.ohs + d, x);
+        if (w.n == 1) store4<DT>(a.out, p.t * a.ors + p.head * a.ohs + d, x);
         else *reinterpret_cast<float4 *>(a.po + p.at * D + d) = x;
     };
     float *s_j = reinterpret_cast<float *>(s_buf) + wave * (16 * LJ);
@@ -706,7 +844,7 @@ k_tree_wide(KvView c, AttnArgs a) {
     for (int rb = 0; rb < RB; rb++) {
         const int r0 = row0 + 16 * (RB * wave + rb);
         const float inv = R.l[rb] == 0.0f ? 0.0f : back / R.l[rb];
-        if (a.splits > 1 && g == 0 && r0 + l16 < rows) a.pml[place(r0 + l16).at] = make_float2(R.m[rb], R.l[rb]);
+        if (w.n > 1 && g == 0 && r0 + l16 < rows) a.pml[place(r0 + l16).at] = make_float2(R.m[rb], R.l[rb]);
         Place p[4];
 #pragma unroll
         for (int n = 0; n < 4; n++) p[n] = place(min(r0 + 4 * n + g, rows - 1));
@@ -731,24 +869,25 @@ k_tree_wide(KvView c, AttnArgs a) {
 // channels of a row and head, a thread 4 of them of every 16th split, so that all
 // splits are requested at once (131072 tokens in 128 splits, 48 rows and heads of
 // 256 channels: 4.6 us; a block a row and head, 11.6).
-template <int D, int DT>
+template <int D, int DT, bool DEALT>
 __global__ void __launch_bounds__(256)
 k_tree_join(AttnArgs a, int heads) {
     constexpr int TD = 16, NG = 256 / TD, U = kMaxSplits / NG;
     __shared__ float s_w[kMaxSplits], s_part[NG][4 * TD];
     const int2 sr = seq_rows(a.row_start, (int)blockIdx.z, a.T, a.max_nodes);
-    if ((int)blockIdx.y >= sr.y) return;
+    const int2 parts = parts_of<DEALT>(a, (int)blockIdx.z, sr);
+    if ((int)blockIdx.y >= sr.y || !parts.x) return;
     const int head = (int)blockIdx.x / (D / 64), dl = (int)threadIdx.x % TD * 4, d = (int)blockIdx.x % (D / 64) * 64 + dl, grp = (int)threadIdx.x / TD, lane = threadIdx.x & 63;
     const long t = sr.x + (int)blockIdx.y;
-    const size_t row = (size_t)t * heads + head, step = (size_t)a.T * heads;
+    const size_t row = (size_t)(parts.y + (int)blockIdx.y) * heads + head, step = (size_t)sr.y * heads;
     // every wave finds the weights, two splits a lane
     float2 ml[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) ml[i] = lane + 64 * i < a.splits ? a.pml[(lane + 64 * i) * step + row] : make_float2(kNoMax, 0.0f);
+    for (int i = 0; i < 2; i++) ml[i] = lane + 64 * i < parts.x ? a.pml[(lane + 64 * i) * step + row] : make_float2(kNoMax, 0.0f);
     float4 y[U];
 #pragma unroll
     for (int i = 0; i < U; i++)
-        if (grp + NG * i < a.splits) y[i] = *reinterpret_cast<const float4 *>(a.po + ((grp + NG * i) * step + row) * D + d);
+        if (grp + NG * i < parts.x) y[i] = *reinterpret_cast<const float4 *>(a.po + ((grp + NG * i) * step + row) * D + d);
     float mn = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
     for (int o = 32; o; o >>= 1) mn = fmaxf(mn, __shfl_xor(mn, o));
@@ -780,50 +919,64 @@ k_tree_join(AttnArgs a, int heads) {
     store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
-// The same where the splits are few (up to kFewSplits): a thread 4 channels of
-// a row and head over all splits, 1024 / D rows and heads a block.
+// The same where the splits are few (kFewSplits on average): a thread 4 channels
+// of a row and head over all splits, kFewSplits at a time, 1024 / D rows and heads
+// a block.
 constexpr int kFewSplits = 8;
-template <int D, int DT>
+template <int D, int DT, bool DEALT>
 __global__ void __launch_bounds__(256)
 k_tree_join_few(AttnArgs a, int heads) {
     constexpr int TD = D / 4;
     const int2 sr = seq_rows(a.row_start, (int)blockIdx.z, a.T, a.max_nodes);
+    const int2 parts = parts_of<DEALT>(a, (int)blockIdx.z, sr);
     const int i = (int)blockIdx.x * (256 / TD) + (int)threadIdx.x / TD, node = i / heads, head = i - node * heads;
-    if (node >= sr.y) return;
+    if (node >= sr.y || !parts.x) return;
     const int d = (int)threadIdx.x % TD * 4;
-    const long t = sr.x + node;
-    const size_t row = (size_t)t * heads + head, step = (size_t)a.T * heads;
-    float2 ml[kFewSplits];
-    float4 y[kFewSplits];
-#pragma unroll
-    for (int s = 0; s < kFewSplits; s++) {
-        ml[s] = make_float2(kNoMax, 0.0f);
-        y[s] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (s < a.splits) {
-            ml[s] = a.pml[s * step + row];
-            y[s] = *reinterpret_cast<const float4 *>(a.po + (s * step + row) * D + d);
-        }
-    }
-    float mn = kNoMax, sum = 0.0f;
-#pragma unroll
-    for (int s = 0; s < kFewSplits; s++) mn = fmaxf(mn, ml[s].x);
+    const size_t row = (size_t)(parts.y + node) * heads + head, step = (size_t)sr.y * heads;
+    float m = kNoMax, sum = 0.0f;
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](int s0, bool more) {
+        float2 ml[kFewSplits];
+        float4 y[kFewSplits];
 #pragma unroll
-    for (int s = 0; s < kFewSplits; s++) {
-        const float w = ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - mn);
-        sum += w;
-        // a split without keys wrote no result
-        const bool none = w == 0.0f;
-        x.x = none ? x.x : fmaf(w, y[s].x, x.x); x.y = none ? x.y : fmaf(w, y[s].y, x.y);
-        x.z = none ? x.z : fmaf(w, y[s].z, x.z); x.w = none ? x.w : fmaf(w, y[s].w, x.w);
-    }
+        for (int s = 0; s < kFewSplits; s++) {
+            ml[s] = make_float2(kNoMax, 0.0f);
+            y[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (s0 + s < parts.x) {
+                ml[s] = a.pml[(s0 + s) * step + row];
+                y[s] = *reinterpret_cast<const float4 *>(a.po + ((s0 + s) * step + row) * D + d);
+            }
+        }
+        float mn = m;
+#pragma unroll
+        for (int s = 0; s < kFewSplits; s++) mn = fmaxf(mn, ml[s].x);
+        if (more) {
+            const float old = __builtin_amdgcn_exp2f(m - mn);
+            sum *= old;
+            x.x *= old; x.y *= old; x.z *= old; x.w *= old;
+        }
+        m = mn;
+#pragma unroll
+        for (int s = 0; s < kFewSplits; s++) {
+            const float w = ml[s].y * __builtin_amdgcn_exp2f(ml[s].x - mn);
+            sum += w;
+            // a split without keys wrote no result
+            const bool none = w == 0.0f;
+            x.x = none ? x.x : fmaf(w, y[s].x, x.x); x.y = none ? x.y : fmaf(w, y[s].y, x.y);
+            x.z = none ? x.z : fmaf(w, y[s].z, x.z); x.w = none ? x.w : fmaf(w, y[s].w, x.w);
+        }
+    };
+    add(0, false);
+    if constexpr (DEALT)
+        for (int s0 = kFewSplits; s0 < parts.x; s0 += kFewSplits) add(s0, true);
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    store4<DT>(a.out, t * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    store4<DT>(a.out, (long)(sr.x + node) * a.ors + head * a.ohs + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
 // How a call is laid out: 16 rb rows a wave, in k_tree_attn or k_tree_wide, and
 // the splits of a sequence's keys.
-struct AttnPlan { int rb, block, splits; bool wide; };      // block: rows a workgroup
+// block: rows a workgroup; slots: workgroups along the keys for a head's block of rows
+struct AttnPlan { int rb, block, splits, slots; bool wide; };
 // what a wave holds within 256 registers
 constexpr int few_blocks(int D, bool f32) { return D == 256 && f32 ? 1 : 2; }
 constexpr int wide_blocks(int D, bool f32) { return D == 64 || (D == 128 && !f32) ? 2 : 1; }
@@ -835,10 +988,10 @@ constexpr int few_resident(int D, int rb) { return rb == 1 ? (D == 64 ? 3 : 2) :
 // resident workgroups (fractions of one for the most part: sequences differ in
 // length), each a prologue and its tiles; a step is as long as its loads' latency
 // or as what the CU's workgroups compute together; a join and its partial results.
-// What it picks takes 1.3% more than the best layout on average; one round of
-// resident workgroups with the widest rows took 22% more. Each form is there for
-// what the others lose without it: 16 rows a wave 17%, 32 rows 4%, k_tree_wide 3%
-// (61-node trees of five users: 84 us, 75 with it before its waves were offset).
+// What it picks takes 1.2% more than the best layout on average; one round of
+// resident workgroups with the widest rows took 21% more. Each form is there for
+// what the others lose without it: 16 rows a wave 16%, 32 rows 3%, k_tree_wide 3%
+// (61-node trees of five users: 84 us, 75 with it, before the keys were dealt out).
 static float attn_cost(const AttnPlan &p, int D, int dtype, long groups, int rows, long tiles) {
     const float d = D / 128.0f, each = p.wide ? 1 : kAttnWaves;
     const bool f32 = dtype == QFM_DT_F32, f16 = dtype == QFM_DT_F16;
@@ -853,6 +1006,18 @@ static float attn_cost(const AttnPlan &p, int D, int dtype, long groups, int row
     float us = 3.9f + rounds * ((p.wide ? 2.2f : 1.1f) + 1.1f * d * p.rb + steps * step);
     if (p.splits > 1) us += 3.1f + (p.splits > kFewSplits ? 1.4f : 0.0f) + (float)all * std::min(p.block, rows) * D * 8 / 5.4e6f;
     return us;
+}
+
+// whether the keys of so many sequences may be dealt out by length
+static bool dealt_seqs(int n_seq) { return n_seq > 1 && n_seq <= kDealSeqs; }
+
+// What is left of the CUs, all of them or each a further time, is dealt out, too.
+static void attn_slots(AttnPlan &p, int kv_heads, int n_seq, int rows) {
+    p.slots = n_seq * p.splits;
+    if (p.splits == 1 || !dealt_seqs(n_seq)) return;
+    const long groups = (long)kv_heads * ((rows + p.block - 1) / p.block);
+    const long fill = (groups * p.slots + 255) / 256 * 256 / groups;
+    p.slots = (int)std::min<long>(std::max<long>(p.slots, fill), (long)n_seq * (p.splits + 1) - 1);
 }
 
 static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_nodes, int max_ctx, int dtype) {
@@ -880,6 +1045,9 @@ static AttnPlan attn_plan(int D, int kv_heads, int n_seq, int q_heads, int max_n
             }
         }
     }
+    // half the work may be one sequence's: a second workgroup for it where a join is little beside that
+    if (best.splits == 1 && dealt_seqs(n_seq) && least > 100.0f && tiles > 1) best.splits = 2;
+    attn_slots(best, kv_heads, n_seq, rows);
     return best;
 }
 
@@ -891,8 +1059,14 @@ static int attn_shape(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int 
     return (long)c->kv_heads * ((max_nodes * (q_heads / c->kv_heads) + 15) / 16) > 65535 ? -1 : 0;
 }
 
-static size_t attn_ws(const qfm_kv_cache *c, int splits, int T, int q_heads) {
-    return splits == 1 ? 0 : (size_t)splits * T * q_heads * (c->head_dim + 2) * 4;
+// rows of partial results: every split of a sequence has all its rows
+static long attn_rows(const AttnPlan &p, int n_seq, int T, int max_nodes) {
+    if (p.splits == 1) return 0;
+    const long even = (long)p.splits * T;
+    return dealt_seqs(n_seq) ? std::max(even, std::min((long)p.slots * max_nodes, std::min<long>(p.slots, kMaxSplits) * T)) : even;
+}
+static size_t attn_ws(const qfm_kv_cache *c, long rows, int n_seq, int q_heads) {
+    return rows ? (size_t)rows * q_heads * (c->head_dim + 2) * 4 + (size_t)n_seq * 8 : 0;
 }
 
 template <int FMT, int D, int DT>
@@ -904,20 +1078,26 @@ static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, d
     else if (p.rb == 1) hipLaunchKernelGGL((k_tree_attn<FMT, D, 1, DT>), g, b, 0, s, v, a);
     else if constexpr (few_blocks(D, F32) == 2) hipLaunchKernelGGL((k_tree_attn<FMT, D, 2, DT>), g, b, 0, s, v, a);
 }
+template <int D, int DT, bool DEALT>
+static void attn_join(const AttnArgs &a, int heads, int n_seq, hipStream_t s) {
+    if (a.splits <= kFewSplits) {
+        const dim3 gj((unsigned)((heads * a.max_nodes + 1024 / D - 1) / (1024 / D)), 1, (unsigned)n_seq);
+        hipLaunchKernelGGL((k_tree_join_few<D, DT, DEALT>), gj, dim3(256), 0, s, a, heads);
+    } else {
+        const dim3 gj((unsigned)(heads * (D / 64)), (unsigned)a.max_nodes, (unsigned)n_seq);
+        hipLaunchKernelGGL((k_tree_join<D, DT, DEALT>), gj, dim3(256), 0, s, a, heads);
+    }
+}
 template <int D, int DT>
 static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, int fmt, int n_seq, hipStream_t s) {
     const int rows = a.max_nodes * a.G, heads = v.heads * a.G;
-    const dim3 g((unsigned)a.splits, (unsigned)(v.heads * ((rows + p.block - 1) / p.block)), (unsigned)n_seq);
+    const dim3 g((unsigned)(a.dealt ? p.slots : p.splits), (unsigned)(v.heads * ((rows + p.block - 1) / p.block)),
+                 a.dealt ? 1u : (unsigned)n_seq);
     if (fmt == QFM_KV_INT8) attn_launch<QFM_KV_INT8, D, DT>(v, a, p, g, s);
     else attn_launch<QFM_KV_E4M3, D, DT>(v, a, p, g, s);
     if (a.splits == 1) return;
-    if (a.splits <= kFewSplits) {
-        const dim3 gj((unsigned)((heads * a.max_nodes + 1024 / D - 1) / (1024 / D)), 1, (unsigned)n_seq);
-        hipLaunchKernelGGL((k_tree_join_few<D, DT>), gj, dim3(256), 0, s, a, heads);
-    } else {
-        const dim3 gj((unsigned)(heads * (D / 64)), (unsigned)a.max_nodes, (unsigned)n_seq);
-        hipLaunchKernelGGL((k_tree_join<D, DT>), gj, dim3(256), 0, s, a, heads);
-    }
+    if (a.dealt) attn_join<D, DT, true>(a, heads, n_seq, s);
+    else attn_join<D, DT, false>(a, heads, n_seq, s);
 }
 template <int D>
 static void attn_launch(const KvView &v, const AttnArgs &a, const AttnPlan &p, int dtype, int fmt, int n_seq, hipStream_t s) {
@@ -934,10 +1114,10 @@ extern "C" {
 
 size_t qfm_tree_attn_ws_bytes(const qfm_kv_cache *c, int n_seq, int T, int q_heads, int max_nodes, int max_ctx) {
     if (attn_shape(c, n_seq, T, q_heads, max_nodes, max_ctx)) return 0;
-    int splits = 1;
+    long rows = 0;
     for (int dtype : {QFM_DT_F32, QFM_DT_BF16, QFM_DT_F16})
-        splits = std::max(splits, attn_plan(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, dtype).splits);
-    return attn_ws(c, splits, T, q_heads);
+        rows = std::max(rows, attn_rows(attn_plan(c->head_dim, c->kv_heads, n_seq, q_heads, max_nodes, max_ctx, dtype), n_seq, T, max_nodes));
+    return attn_ws(c, rows, n_seq, q_heads);
 }
 
 int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, void *out, int dtype, int q_heads,
@@ -970,17 +1150,28 @@ int qfm_tree_attn(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *q, v
     if (!(scale > 0.0f) || !(scale < 3.4e38f)) { set_error(-1, "%s: scale %g", who, (double)scale); return -1; }
     const int D = c->head_dim, G = q_heads / c->kv_heads;
     const AttnPlan p = attn_plan(D, c->kv_heads, sq->n_seq, q_heads, max_nodes, max_ctx, dtype);
-    const int splits = p.splits;
-    const size_t need = attn_ws(c, splits, T, q_heads);
+    const long rows = attn_rows(p, sq->n_seq, T, max_nodes);
+    const size_t need = attn_ws(c, rows, sq->n_seq, q_heads);
     if (need && (!ws || ws_bytes < need || reinterpret_cast<uintptr_t>(ws) & 15)) {
         set_error(-1, "%s: workspace of %zu bytes (16-byte aligned), %zu needed", who, ws ? ws_bytes : (size_t)0, need);
         return -1;
     }
     if (T == 0) return 0;
-    AttnArgs a{static_cast<const uint8_t *>(q), static_cast<uint8_t *>(out), G, T, max_nodes, splits,
-               q_row_stride, q_head_stride, out_row_stride, out_head_stride, row_start, ctx, tree, scale, nullptr, nullptr};
-    a.po = static_cast<float *>(ws);
-    if (splits > 1) a.pml = reinterpret_cast<float2 *>(a.po + (size_t)splits * T * q_heads * D);
+    AttnArgs a{};
+    a.q = static_cast<const uint8_t *>(q);
+    a.out = static_cast<uint8_t *>(out);
+    a.G = G; a.T = T; a.max_nodes = max_nodes; a.splits = p.splits;
+    a.qrs = q_row_stride; a.qhs = q_head_stride; a.ors = out_row_stride; a.ohs = out_head_stride;
+    a.row_start = row_start; a.ctx = ctx; a.tree = tree; a.scale = scale;
+    if (p.splits > 1) {
+        // (the sum of all tiles stays an int)
+        const long most = (std::min((long)sq->max_pages * c->page, kMaxTokens) >> 5) + 1;
+        a.dealt = dealt_seqs(sq->n_seq) && most * sq->n_seq < 1l << 31;
+        a.rows = (int)rows;
+        a.po = static_cast<float *>(ws);
+        a.pml = reinterpret_cast<float2 *>(a.po + (size_t)rows * q_heads * D);
+        a.parts = reinterpret_cast<int2 *>(a.pml + (size_t)rows * q_heads);
+    }
     if (D == 64) attn_launch<64>(v, a, p, dtype, c->fmt, sq->n_seq, s);
     else if (D == 128) attn_launch<128>(v, a, p, dtype, c->fmt, sq->n_seq, s);
     else attn_launch<256>(v, a, p, dtype, c->fmt, sq->n_seq, s);

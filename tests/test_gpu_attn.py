@@ -134,6 +134,27 @@ def test_every_layout(seqs, m, Hq, H, max_ctx, D, dt, fmt):
     _run(rng, c, counts, ctx, Hq, dt, max_ctx=max_ctx, max_nodes=m, extra=1)
 
 
+@pytest.mark.parametrize("seqs,long_one,Hq,H,D,dt,max_ctx", [
+    (2, 3000, 8, 2, 64, "bf16", 3000), (5, 4000, 16, 1, 128, "f16", 4000), (37, 2500, 8, 4, 64, "f32", 131071),
+    (70, 2000, 4, 2, 128, "bf16", 4000),                    # more sequences than lanes
+    (200, 1500, 4, 1, 64, "bf16", 100000), (256, 700, 4, 1, 256, "f32", 100000),
+    (257, 700, 4, 1, 64, "f16", 100000), (300, 300, 2, 1, 64, "bf16", 9000)])
+def test_one_long_sequence_among_short_ones(seqs, long_one, Hq, H, D, dt, max_ctx):
+    """The keys are dealt out by length: sequences in one part, in several and without rows beside each other, the long
+    one anywhere; and a batch in which nobody has rows."""
+    _say(seqs, "sequences, one of", long_one, "heads", Hq, H, "D", D, dt, "planned for", max_ctx)
+    rng = np.random.default_rng(seqs)
+    for at in (0, seqs // 2, seqs - 1):
+        ctx = [int(x) for x in rng.integers(0, 40, seqs)]
+        counts = [int(x) for x in rng.integers(0, 3, seqs)]
+        ctx[at], counts[at] = long_one, 3
+        ctx[(at + 1) % seqs] = long_one // 2
+        c = _pool(rng, [a + b for a, b in zip(ctx, counts)], 16, H, D, E4M3)
+        _run(rng, c, counts, ctx, Hq, dt, max_ctx=max_ctx, max_nodes=4, extra=2)
+    c = _pool(rng, [1] * seqs, 16, H, D, INT8)
+    _run(rng, c, [0] * seqs, [0] * seqs, Hq, dt, max_ctx=max_ctx, max_nodes=4, extra=3)
+
+
 @pytest.mark.parametrize("D,dt", [(128, "bf16"), (256, "f16"), (64, "f32")])
 def test_chain_and_rows_of_no_sequence(D, dt):
     """No masks: a chain. Rows behind the last sequence, and a sequence without rows, are left alone."""
