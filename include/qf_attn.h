@@ -93,8 +93,10 @@ int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, 
  *           dtype; strides multiples of 8 and not negative (out: at least D),
  *           16-byte aligned. Rows of out that no sequence has are left.
  *   T       rows of q; row_start beyond it is cut there
- *   max_ctx the largest ctx the host expects: it sets how far a sequence's keys
- *           are split over the GPU, nothing else (longer ones are right, too)
+ *   max_ctx the largest ctx the host expects: it sets how many workgroups the
+ *           keys are split over, nothing else (longer ones are right, too). Up to
+ *           256 sequences share them by length, so that where the sums of one are
+ *           split, and how they round, depends on the others' lengths.
  *   scale   > 0
  *   ws      at least qfm_tree_attn_ws_bytes of the same arguments, 16-byte
  *           aligned, no initialisation; calls that share it must not overlap.
