@@ -734,8 +734,8 @@ k_tree_wide(KvView c, AttnArgs a) {
                 dst += (4 * NC + 4 * k) * 1024 + 8 * i;
                 *reinterpret_cast<u32x2_t *>(dst) = u32x2_t{p[0], p[1]};
                 *reinterpret_cast<u32x2_t *>(dst + 1024) = u32x2_t{p[2], p[3]};
-                *reinterpret_cast<u32x2_t *>(dst + 2048) = u32x2_t{q[0], q[1]};
-                *reinterpret_cast<u32x2_t *>(dst + 3072) = u32x2_t{q[2], q[3]};
+                *reinterpret_cast<u32x2_t *>(dst + 2 * 1024) = u32x2_t{q[0], q[1]};
+                *reinterpret_cast<u32x2_t *>(dst + 3 * 1024) = u32x2_t{q[2], q[3]};
             }
         }
         if (wave == 0) s_sc[tt & 1][lane] = raw_sc;
