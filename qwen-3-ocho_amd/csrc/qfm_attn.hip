@@ -26,8 +26,7 @@
 // The bound of a large call is its cache: 37 users of 2 to 4 thousand tokens,
 // 124 MB of codes and scales, take 33.0 us (3.8 TB/s, a plain sum over as much
 // memory reads 4.0). Many rows a head are bound by the softmax between the two
-// products, 16 rows by 32 tokens of which cost a wave about as long as their
-// MFMAs (61-node trees of five users, 26 GFLOP: 64 us; k_tree_wide below). Few
+// products, which costs a wave about half as long again as their MFMAs (61-node trees of five users, 26 GFLOP: 64 us; k_tree_wide below). Few
 // rows and short contexts are bound by the chain of a launch, the page table,
 // the first tile, a join through LDS and one through memory (1021 tokens: 9.8
 // us); what is there to fill the GPU is the split of the keys.
