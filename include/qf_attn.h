@@ -36,7 +36,7 @@ extern "C" {
 #define QFM_DT_F16  2
 
 /* A layer's pool of pages. page: tokens a page, 16, 32, 64, 128 or 256;
- * head_dim D: 64, 128 or 256.
+ * head_dim D: 64, 128 or 256; kv_heads up to 1024.
  *   k  codes [n_pages][kv_heads][page][D]
  *   v  codes [n_pages][kv_heads][page / 4][D][4]: four tokens of one channel
  *      side by side, so that attention's second product, whose inner dimension
@@ -52,7 +52,7 @@ typedef struct {
 /* The sequences' pages: position p of sequence s lies in page
  * table[s][p / page] (device, int32 [n_seq][max_pages]) at token p % page. A
  * page id outside [0, n_pages) is no page: rows there are neither written nor
- * read, and attention does not see them. */
+ * read, and attention does not see them. Up to 65535 sequences. */
 typedef struct {
     const int *table;
     int        n_seq, max_pages;
@@ -61,7 +61,7 @@ typedef struct {
 /* T rows of keys and values (k and v: element (t, h, d) at t * row_stride +
  * h * head_stride + d, type dtype) into positions pos[t] of the sequences
  * seq[t] (device int32 [T]). Strides are multiples of 8 and not negative, k and
- * v 16-byte aligned. A row whose sequence, position or page does not exist
+ * v 16-byte aligned, T up to 2^24. A row whose sequence, position or page does not exist
  * (pos -1, say) is passed over. Rows of one call name different places: of two
  * that name the same one, codes and scale may be from either. */
 int qfm_kv_write(const qfm_kv_cache *c, const qfm_kv_seqs *sq, const void *k, const void *v, int dtype,
@@ -92,7 +92,9 @@ int qfm_kv_read(const qfm_kv_cache *c, const qfm_kv_seqs *sq, void *k, void *v, 
  *   q, out  element (t, h, d) at t * row_stride + h * head_stride + d, type
  *           dtype; strides multiples of 8 and not negative (out: at least D),
  *           16-byte aligned. Rows of out that no sequence has are left.
- *   T       rows of q; row_start beyond it is cut there
+ *   T       rows of q, up to 2^22; row_start beyond it is cut there
+ *   q_heads a multiple of kv_heads, up to 4096; kv_heads times the blocks of 16
+ *           rows that max_nodes q_heads / kv_heads rows make, up to 65535
  *   max_ctx the largest ctx the host expects: it sets how many workgroups the
  *           keys are split over, nothing else (longer ones are right, too). Up to
  *           256 sequences share them by length, so that where the sums of one are
