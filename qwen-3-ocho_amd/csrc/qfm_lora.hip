@@ -14,7 +14,7 @@
 //
 // What it has to move is base and y (8 bytes an output and row), x and the
 // adapters in use: 97.5 MB for 2050 rows of K 2048 to 4096 + 512 + 512 outputs at
-// rank 64, of which k_lora_in takes 16.5 us and k_lora_out 28 (3.0 TB/s). A decode
+// rank 64, of which k_lora_in takes 16.4 us and k_lora_out 22.6 (3.7 TB/s). A decode
 // batch is bound by the chain launch, slots, A and x, sums, launch, h, B, base
 // (37 rows of 24 adapters, 7 MB: 11.3 us).
 #include "qfm_dev.h"
@@ -332,7 +332,10 @@ k_lora_out(LoraArgs a, LoraFirst first, int NB) {
             if (!(rows >> (4 * q + g) & 1) || oc >= N) continue;
             const float4 v = make_float4(bs[q][0] + d.x, bs[q][1] + d.y, bs[q][2] + d.z, bs[q][3] + d.w);
             float *y = a.y[i] + (size_t)(16 * blk + 4 * q + g) * N + oc;
-            if (whole) {
+            if (whole && !EACH) {
+                // more than the caches keep: past them (2050 rows 44.1 -> 38.1 us; with a reader of y behind it 61.2 -> 60.4)
+                __builtin_nontemporal_store(f32x4_t{v.x, v.y, v.z, v.w}, reinterpret_cast<f32x4_t *>(y));
+            } else if (whole) {
                 *reinterpret_cast<float4 *>(y) = v;
             } else {
                 y[0] = v.x;
